@@ -37,6 +37,49 @@ int projection_rows(const FryNetwork* n, int dq) {
     return (n->heads + n->kv_heads) * dq + n->kv_heads * n->dv + n->heads * n->templates_count;
 }
 
+fry::AttentionShape packed_shape(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim) {
+    fry::AttentionShape s;
+    s.q_rows = q_rows, s.key_rows = k_rows, s.sequences = sequences, s.heads = heads, s.kv_heads = kv_heads, s.width = head_dim;
+    return s;
+}
+
+fry::AttentionShape cached_shape(int sequences, int capacity, int heads, int kv_heads, int head_dim) {
+    fry::AttentionShape s = packed_shape(sequences, capacity, sequences, heads, kv_heads, head_dim);
+    s.capacity = capacity;
+    s.cached = true;
+    return s;
+}
+
+// Why the attention kernels do not take a shape ("" if they do). key_rows is the capacity for a cache.
+std::string attention_refusal(const fry::AttentionShape& s) {
+    if (s.q_rows < 0 || s.key_rows < 0 || s.sequences < 0) return "needs row and sequence counts >= 0";
+    if (s.kv_heads <= 0 || s.heads <= 0 || s.heads > 1024 || s.heads % s.kv_heads != 0)
+        return "takes 1 to 1024 query heads, a multiple of the key/value heads, got " + std::to_string(s.heads) + " and " + std::to_string(s.kv_heads);
+    if (s.width <= 0 || s.width > 128 || s.width % 8 != 0) return "takes heads a multiple of 8 up to 128 wide, got " + std::to_string(s.width);
+    if (s.q_rows > (1 << 26) || s.sequences > (1 << 26)) return "takes up to 2^26 query rows and sequences";
+    return "";
+}
+
+int run_attention(const char* name, const fry::AttentionShape& shape, const fry::AttentionTensors& x, float scale, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    std::string refusal = attention_refusal(shape);
+    if (refusal.empty() && !(scale > 0.0f && scale <= 3.0e38f)) refusal = "takes a positive, finite scale";
+    if (refusal.empty()) {
+        for (int64_t stride : {x.q_row, x.q_head, x.k_row, x.k_head, x.v_row, x.v_head, x.k_sequence, x.v_sequence})
+            if (stride < 0 || stride % 8 != 0) refusal = "takes strides of a multiple of 8 elements";
+        if (!aligned16(x.q) || !aligned16(x.k) || !aligned16(x.v) || !aligned16(x.out) || !aligned16(workspace))
+            refusal = "needs 16-byte aligned q, k, v, out and workspace";
+    }
+    if (!refusal.empty()) return fail(FRY_ERROR_SHAPE, std::string(name) + " " + refusal);
+    if (shape.q_rows == 0) return check(cudaSuccess, "");
+    if (!x.q || !x.out || (shape.key_rows > 0 && (!x.k || !x.v)) || (shape.cached ? !x.lengths : !x.q_offsets || !x.k_offsets))
+        return fail(FRY_ERROR_SHAPE, std::string(name) + " needs q, k, v, out and its offsets or lengths");
+    const size_t needed = fry::attention_plan(shape).workspace_bytes;
+    if (needed > 0 && (!workspace || workspace_bytes < needed))
+        return fail(FRY_ERROR_SHAPE, std::string(name) + "'s workspace is smaller than " + name + "_workspace_bytes");
+    return check(fry::packed_attention(shape, x, scale, workspace, as_stream(stream)), name);
+}
+
 constexpr int kAnswerWidth = 1969;  // 1968 move logits, then the expected score
 constexpr uint64_t kMaxWaitLimitNs = 60000000000ull;  // the largest wait limit fry_set_wait_limit_ns takes: 60 s
 
@@ -299,6 +342,46 @@ int fry_attention_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
         return fail(FRY_ERROR_SHAPE, "fry_attention_bf16 needs 16-byte aligned q, k, v and out");
     std::string detail;
     return check(fry::attention64(q, k, v, out, B, heads, as_stream(stream), &detail), "fry_attention_bf16", detail);
+}
+
+size_t fry_packed_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim) {
+    const fry::AttentionShape shape = packed_shape(q_rows, k_rows, sequences, heads, kv_heads, head_dim);
+    return attention_refusal(shape).empty() ? fry::attention_plan(shape).workspace_bytes : 0;
+}
+
+int fry_packed_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int32_t* q_offsets,
+                         const int32_t* k_offsets, int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim,
+                         int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                         int64_t v_head_stride, float scale, int causal, int bf16, void* workspace, size_t workspace_bytes, void* stream) {
+    fry::AttentionShape shape = packed_shape(q_rows, k_rows, sequences, heads, kv_heads, head_dim);
+    shape.causal = causal != 0;
+    shape.bf16 = bf16 != 0;
+    fry::AttentionTensors x;
+    x.q = q, x.k = k, x.v = v, x.out = out;
+    x.q_offsets = q_offsets, x.k_offsets = k_offsets;
+    x.q_row = q_row_stride, x.q_head = q_head_stride, x.k_row = k_row_stride, x.k_head = k_head_stride;
+    x.v_row = v_row_stride, x.v_head = v_head_stride;
+    return run_attention("fry_packed_attention", shape, x, scale, workspace, workspace_bytes, stream);
+}
+
+size_t fry_cached_attention_workspace_bytes(int sequences, int capacity, int heads, int kv_heads, int head_dim) {
+    const fry::AttentionShape shape = cached_shape(sequences, capacity, heads, kv_heads, head_dim);
+    return attention_refusal(shape).empty() ? fry::attention_plan(shape).workspace_bytes : 0;
+}
+
+int fry_cached_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int32_t* lengths, int sequences,
+                         int capacity, int heads, int kv_heads, int head_dim, int64_t q_row_stride, int64_t q_head_stride,
+                         int64_t k_sequence_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_sequence_stride,
+                         int64_t v_row_stride, int64_t v_head_stride, float scale, int bf16, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+    fry::AttentionShape shape = cached_shape(sequences, capacity, heads, kv_heads, head_dim);
+    shape.bf16 = bf16 != 0;
+    fry::AttentionTensors x;
+    x.q = q, x.k = k, x.v = v, x.out = out;
+    x.lengths = lengths;
+    x.q_row = q_row_stride, x.q_head = q_head_stride, x.k_row = k_row_stride, x.k_head = k_head_stride;
+    x.v_row = v_row_stride, x.v_head = v_head_stride, x.k_sequence = k_sequence_stride, x.v_sequence = v_sequence_stride;
+    return run_attention("fry_cached_attention", shape, x, scale, workspace, workspace_bytes, stream);
 }
 
 int fry_norm_quant(const uint16_t* x, const uint16_t* gain, float eps, int8_t* q, float* scale, int M, int D, void* stream) {

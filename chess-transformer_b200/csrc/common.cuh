@@ -26,6 +26,7 @@ enum DeviceError : int {
     kMisaligned = 4,       // dynamic shared memory did not start on the 1024-byte boundary a kernel lays out from
     kBadColumn = 5,        // a lean lane's answer column outside the answer row
     kNotPositiveDefinite = 6,  // a GPTQ Cholesky factorization met a pivot that is not positive (where: the column)
+    kBadOffsets = 7,       // a request's offsets, length or adapter outside its tensors (where: the request)
 };
 
 // Set by kernels on a failure they can detect; read and cleared by fry_device_status(). The library is one

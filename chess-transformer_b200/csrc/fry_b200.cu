@@ -4,6 +4,7 @@
 #include "rows.cu"
 #include "attention.cu"
 #include "attention64.cu"
+#include "packed_attention.cu"
 #include "heads.cu"
 #include "gptq.cu"
 #include "health.cu"

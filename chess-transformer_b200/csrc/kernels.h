@@ -92,6 +92,30 @@ cudaError_t template_attention(const uint16_t* projected, const uint16_t* paired
 cudaError_t attention64(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int B, int heads, cudaStream_t stream,
                         std::string* error);
 
+// Attention over packed sequences and over a cache (packed_attention.cu). Strides in elements; 16-bit rows dense.
+struct AttentionShape {
+    int q_rows = 0, key_rows = 0, sequences = 0, heads = 0, kv_heads = 0, width = 0;
+    int capacity = 0;  // cached: keys a sequence has room for (key_rows is the same)
+    bool cached = false, causal = false, bf16 = false;
+};
+struct AttentionTensors {
+    const uint16_t *q = nullptr, *k = nullptr, *v = nullptr;
+    uint16_t* out = nullptr;
+    const int32_t *q_offsets = nullptr, *k_offsets = nullptr;  // packed: [sequences + 1]
+    const int32_t* lengths = nullptr;                          // cached: [sequences]
+    int64_t q_row = 0, q_head = 0, k_row = 0, k_head = 0, v_row = 0, v_head = 0, k_sequence = 0, v_sequence = 0;
+};
+// What the host chooses from the shape alone: the form, into how many blocks a row's keys are split, and the workspace
+// (the splits' partial results; 0 without a split).
+constexpr int kMaxAttentionSplits = 64;
+struct AttentionPlan {
+    bool few = false;
+    int splits = 1;
+    size_t workspace_bytes = 0;
+};
+AttentionPlan attention_plan(const AttentionShape& shape);
+cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& tensors, float scale, void* workspace, cudaStream_t stream);
+
 // Heads (heads.cu).
 struct HeadWeights {
     const uint16_t* ln_gain;         // fp16 [d]

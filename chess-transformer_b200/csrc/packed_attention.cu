@@ -1,0 +1,516 @@
+// Attention over packed sequences and over a cache, on warp-wide tensor steps (mma.sync): out = softmax(scale q k^T) v for
+// each token and head, grouped heads (query head h reads key/value head h / group), causal or not.
+//
+//  packed: q [rows, heads, width], k and v [key rows, kv_heads, width], sequences one behind the other at q_offsets and
+//          k_offsets. Causal: a sequence's queries are its last tokens, query i sees keys j <= i + nk - nq.
+//  cached: q [sequences, heads, width], one token a sequence, k and v [sequences, capacity, kv_heads, width] of which the
+//          first lengths[s] keys count.
+//
+// Softmax in one pass over the keys: with m the running maximum of a row's scores (times scale log2 e) and l the running
+// sum of 2^(s - m), a tile of keys takes m to m' = max(m, its maximum), scales l and the row's sums o by 2^(m - m') and
+// adds its own 2^(s - m') and 2^(s - m') v. out = o / l at the end; a row that sees no key has l = 0 and answers 0. Scores,
+// m, l and o are fp32. The probabilities 2^(s - m') are rounded to the inputs' type for the second product (off by at most
+// half a step each, about what rounding the output costs), l sums them unrounded.
+//
+// Rows. The `group` query heads of a key/value head share its keys, so they are rows of one tile: row r of a block is token
+// r / group, head r % group, and one pass over the keys serves them all.
+//
+// Two forms. ROW_WARPS warps of 16 rows each share tiles of keys (many queries), or KEY_WARPS warps hold the same 16 rows
+// and take different keys, each with copies and a softmax of its own, joined at the end (few queries: there the loads
+// bound the kernel, and warps that wait for no other keep them in flight). Where blocks are still fewer than the SMs, the
+// keys are also split over blocks (`splits`): each writes its m, l and o to a workspace and attention_join_kernel joins
+// them in order of the split, so results do not depend on the blocks' order.
+//
+// What a query does not see does not reach it, whatever it holds: scores behind a row's last key count as -inf however
+// they came out, and rows behind a sequence's last key are read as zeros. A value of a key that some rows of a tile see
+// and others do not is multiplied by their probability 0; if it is not finite that product is NaN, so a row whose sum l is
+// finite and whose output is not is computed again over its own keys alone (recompute_row).
+#include <climits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "segments.cuh"
+
+namespace fry {
+
+struct AttentionArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;                                         // [rows, heads, width] dense
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
+    int64_t k_sequence, v_sequence;                        // cached
+    int heads, kv_heads, width;
+    int group, tile_heads, head_tiles;  // query heads a key/value head, of which a block takes tile_heads in each of head_tiles
+    PackedRows queries;                 // packed; cached: count sequences of one row
+    const int32_t* k_offsets;           // packed: [count + 1]
+    int k_rows;
+    const int32_t* lengths;             // cached: [count], else null
+    int capacity;
+    int causal;
+    float scale_log2;                   // scale * log2(e), positive
+    int splits;
+    float* part_out;                    // [splits][rows][heads][width], where splits > 1
+    float* part_sums;                   // [splits][rows][heads][2]: m, l
+};
+
+// A block's rows: tokens [first, first + tokens) of a sequence of nq queries and nk keys.
+struct RowBlock {
+    int row;     // the first token's row of q and out
+    int first, tokens, nq, nk;
+    int64_t k_base, v_base;  // the sequence's first key and value, in elements
+    FRY_DEVICE int limit(int token, int causal) const {  // how many keys a token sees
+        if (!causal) return nk;
+        const int seen = nk - nq + first + token + 1;
+        return seen < 0 ? 0 : seen > nk ? nk : seen;
+    }
+};
+
+// The rows of block `slot` of tiles of `tile` tokens; false if it has none. Every thread of the warp calls it.
+FRY_DEVICE bool find_rows(const AttentionArgs& a, int tile, int slot, int lane, RowBlock& b) {
+    b.k_base = b.v_base = 0;
+    if (a.lengths) {
+        if (slot >= a.queries.count) return false;
+        const int length = a.lengths[slot];
+        b.row = slot, b.first = 0, b.tokens = 1, b.nq = 1;
+        b.nk = length < 0 ? 0 : length > a.capacity ? a.capacity : length;
+        if (b.nk != length && threadIdx.x == 0) record_error(kBadOffsets, slot);
+        b.k_base = slot * a.k_sequence, b.v_base = slot * a.v_sequence;
+        return true;
+    }
+    const int segment = find_segment(a.queries, tile, slot, lane);
+    const int start = a.queries.start(segment), end = a.queries.start(segment + 1);
+    b.first = (slot - start / tile - segment) * tile;
+    b.nq = end > start ? end - start : 0;
+    b.tokens = min(tile, b.nq - b.first);
+    if (b.tokens <= 0) return false;
+    b.row = start + b.first;
+    b.nk = 0;
+    if (segment >= 1 && segment <= a.queries.count) {  // not the rows before the first or behind the last sequence
+        const PackedRows keys{a.k_offsets, a.queries.count, a.k_rows};
+        const int k_start = keys.start(segment), k_end = keys.start(segment + 1);
+        b.nk = k_end > k_start ? k_end - k_start : 0;
+        b.k_base = k_start * a.k_row, b.v_base = k_start * a.v_row;
+    }
+    return true;
+}
+
+// Records a sequence whose offsets descend or leave their tensor. One block of a launch does it for all, the first: it has
+// the rows behind the last sequence, usually none.
+FRY_DEVICE void check_offsets(const AttentionArgs& a) {
+    if (a.lengths || blockIdx.x != 0 || blockIdx.y != 0 || blockIdx.z != 0) return;
+    const PackedRows keys{a.k_offsets, a.queries.count, a.k_rows};
+    for (int s = threadIdx.x; s < a.queries.count; s += blockDim.x)
+        if (a.queries.bad(s + 1) || keys.bad(s + 1)) record_error(kBadOffsets, s);
+}
+
+template <bool BF16>
+FRY_DEVICE float widen16(uint16_t bits) {
+    if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+    else return h2f_bits(bits);
+}
+template <bool BF16>
+FRY_DEVICE uint32_t pack16(float lo, float hi) {
+    if constexpr (BF16) return pack_bf162_rn(lo, hi);
+    else return pack_half2_rn(lo, hi);
+}
+template <bool BF16>
+FRY_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) mma_bf16(c, a, b0, b1);
+    else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// Where a row's results go: out (o / l rounded), or with splits this split's m, l and o.
+struct AttentionOut {
+    uint16_t* out;
+    float *part_out, *part_sums;
+};
+FRY_DEVICE AttentionOut attention_out(const AttentionArgs& a, int split, int row, int head) {
+    const int64_t at = static_cast<int64_t>(row) * a.heads + head;
+    const int64_t part = static_cast<int64_t>(split) * a.queries.rows * a.heads + at;
+    return {a.out + at * a.width, a.part_out + part * a.width, a.part_sums + part * 2};
+}
+
+// One row by its definition, by a warp: softmax over keys [low, high) in tiles of 32, lane i summing columns i, i + 32, ...
+// Slow, for rows whose tile holds values that are not finite.
+template <bool BF16>
+__device__ __noinline__ void recompute_row(const AttentionArgs& a, const RowBlock& b, int token, int head, int low, int high, int split, int lane) {
+    const uint16_t* q = a.q + (b.row + token) * a.q_row + head * a.q_head;
+    const uint16_t* k = a.k + b.k_base + (head / a.group) * a.k_head;
+    const uint16_t* v = a.v + b.v_base + (head / a.group) * a.v_head;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = low; j0 < high; j0 += 32) {
+        float s = -INFINITY;
+        if (j0 + lane < high) {
+            s = 0.0f;
+            for (int c = 0; c < a.width; ++c) s = __fmaf_rn(widen16<BF16>(q[c]), widen16<BF16>(k[(j0 + lane) * a.k_row + c]), s);
+            s *= a.scale_log2;
+        }
+        const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.0f : top;
+        const float p = j0 + lane < high ? ex2_approx(s - base) : 0.0f, shrink = ex2_approx(m - base);
+        l = l * shrink + warp_sum(p);
+        m = top;
+        for (int i = 0; i < 4; ++i) o[i] *= shrink;
+        for (int j = 0; j < 32 && j0 + j < high; ++j) {
+            const float pj = __shfl_sync(0xffffffffu, p, j);
+            for (int i = 0; i < 4; ++i)
+                if (lane + 32 * i < a.width) o[i] = __fmaf_rn(pj, widen16<BF16>(v[(j0 + j) * a.v_row + lane + 32 * i]), o[i]);
+        }
+    }
+    const AttentionOut to = attention_out(a, split, b.row + token, head);
+    for (int i = 0; i < 4; ++i) {
+        const int c = lane + 32 * i;
+        if (c >= a.width) continue;
+        if (a.splits > 1) to.part_out[c] = o[i];
+        else to.out[c] = static_cast<uint16_t>(pack16<BF16>(l == 0.0f ? 0.0f : o[i] / l, 0.0f) & 0xffff);
+    }
+    if (a.splits > 1 && lane == 0) to.part_sums[0] = m, to.part_sums[1] = l;
+}
+
+// Byte offset of 16-byte unit `unit` of row `row` in a tile of rows of WIDTH 16-bit values, so that eight rows' equal
+// units lie in different banks: rows of 128 bytes and up swap units by the row within 8, rows of 64 bytes are paired.
+template <int WIDTH>
+FRY_DEVICE uint32_t tile_unit(int row, int unit) {
+    if constexpr (WIDTH >= 64) return static_cast<uint32_t>(row * WIDTH * 2 + ((unit ^ (row & 7)) << 4));
+    else return static_cast<uint32_t>((row >> 1) * 128 + ((((row & 1) * 4 + unit) ^ ((row >> 1) & 7)) << 4));
+}
+// 16 bytes global -> shared, or zeros without reading
+FRY_DEVICE void cp_async16_or_zero(uint32_t shared, const void* global, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(global), "r"(read ? 16 : 0) : "memory");
+}
+
+// WIDTH: the head width padded to 32, 64 or 128 with zeros. KEYS: the keys a warp takes of a stage (all of it with
+// ROW_WARPS, its own share with KEY_WARPS).
+template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES>
+struct RowsShape {
+    static_assert(ROW_WARPS == 1 || KEY_WARPS == 1, "warps share keys or rows");
+    static constexpr int kThreads = ROW_WARPS * KEY_WARPS * 32;
+    static constexpr int kRows = ROW_WARPS * 16;
+    static constexpr int kStageKeys = KEYS * KEY_WARPS;
+    static constexpr int kTileBytes = kStageKeys * WIDTH * 2;  // the keys or the values of a stage
+    static constexpr int kLoopBytes = STAGES * 2 * kTileBytes;
+    // after the loop: a warp's 16 output rows, or with KEY_WARPS its 16 rows of fp32 sums, m and l
+    static constexpr int kJoinBytes = KEY_WARPS > 1 ? KEY_WARPS * 16 * (WIDTH + 2) * 4 : ROW_WARPS * 16 * WIDTH * 2;
+    static constexpr int kSmemBytes = kLoopBytes > kJoinBytes ? kLoopBytes : kJoinBytes;
+};
+
+template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
+__global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_kernel(const __grid_constant__ AttentionArgs a) {
+    using S = RowsShape<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row_warp = KEY_WARPS > 1 ? 0 : warp, key_warp = KEY_WARPS > 1 ? warp : 0;
+    grid_dependency_start();
+    check_offsets(a);
+
+    const int tile = S::kRows / a.tile_heads;  // tokens a block
+    RowBlock b;
+    // later tokens see more keys: they start first
+    if (!find_rows(a, tile, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, b)) return;
+    const int kv_head = blockIdx.y / a.head_tiles, first_head = kv_head * a.group + (blockIdx.y % a.head_tiles) * a.tile_heads;
+    const int heads_here = min(a.tile_heads, (kv_head + 1) * a.group - first_head);
+    // a row's token and head; rows past the block's tokens or heads compute on zeros and are not written
+    auto token_of = [&](int r) { return r / a.tile_heads; };
+    auto head_of = [&](int r) { return first_head + r % a.tile_heads; };
+    auto live = [&](int r) { return r / a.tile_heads < b.tokens && r % a.tile_heads < heads_here; };
+
+    // this block's keys: those its last token sees, of which a split takes whole stages
+    const int seen = b.limit(b.tokens - 1, a.causal);
+    const int stages = (seen + S::kStageKeys - 1) / S::kStageKeys, per_split = (stages + a.splits - 1) / a.splits;
+    const int split = blockIdx.z;
+    const int low = min(seen, split * per_split * S::kStageKeys), high = min(seen, (split + 1) * per_split * S::kStageKeys);
+    const int steps = (high - low + S::kStageKeys - 1) / S::kStageKeys;
+
+    const uint16_t* keys = a.k + b.k_base + kv_head * a.k_head;
+    const uint16_t* values = a.v + b.v_base + kv_head * a.v_head;
+    constexpr int kUnits = WIDTH / 8;
+    const int units = a.width / 8;
+    auto load = [&](int step) {
+        if (step < steps) {
+            uint8_t* stage = smem + (step % STAGES) * 2 * S::kTileBytes;
+            const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + S::kTileBytes;
+            // each loader (the block, or a key warp for itself) copies KEYS rows
+            constexpr int kLoaders = KEY_WARPS > 1 ? 32 : S::kThreads;
+            const int me = KEY_WARPS > 1 ? lane : static_cast<int>(threadIdx.x), from = key_warp * KEYS;
+#pragma unroll
+            for (int i = 0; i < KEYS * kUnits / kLoaders; ++i) {
+                const int at = me + i * kLoaders, row = from + at / kUnits, unit = at % kUnits;
+                const int key = low + step * S::kStageKeys + row;
+                const bool read = key < high && unit < units;
+                cp_async16_or_zero(k_tile + tile_unit<WIDTH>(row, unit), keys + (read ? key * a.k_row + unit * 8 : 0), read);
+                cp_async16_or_zero(v_tile + tile_unit<WIDTH>(row, unit), values + (read ? key * a.v_row + unit * 8 : 0), read);
+            }
+            static_assert(KEYS * kUnits % kLoaders == 0, "every thread copies the same number of units");
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) load(s);
+
+    // the queries' fragments: rows g and g + 8 of the warp's 16, columns 2t, 2t + 1 and 8 + 2t, 9 + 2t of each 16
+    uint32_t q[WIDTH / 16][4];
+    int limit[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = row_warp * 16 + g + 8 * half;
+        const bool mine = live(r);
+        limit[half] = mine ? b.limit(token_of(r), a.causal) : INT_MAX;
+        const uint16_t* row = a.q + (mine ? (b.row + token_of(r)) * a.q_row + head_of(r) * a.q_head : 0);
+#pragma unroll
+        for (int s = 0; s < WIDTH / 16; ++s)
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+                q[s][half + 2 * part] = mine && 2 * s + part < units ? *reinterpret_cast<const uint32_t*>(row + s * 16 + part * 8 + 2 * t) : 0u;
+    }
+
+    float o[WIDTH / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int step = 0; step < steps; ++step) {
+        cp_async_wait<STAGES - 2>();
+        if constexpr (KEY_WARPS > 1) __syncwarp();
+        else __syncthreads();
+        load(step + STAGES - 1);  // into the stage read in the step before, which every reader has left
+        const uint32_t k_tile = smem_addr(smem + (step % STAGES) * 2 * S::kTileBytes), v_tile = k_tile + S::kTileBytes;
+        float s[KEYS / 8][4] = {};
+        const int key_row = key_warp * KEYS + (lane >> 4) * 8 + (lane & 7), key_unit = (lane >> 3) & 1;
+#pragma unroll
+        for (int n = 0; n < KEYS / 16; ++n)
+#pragma unroll
+            for (int c = 0; c < WIDTH / 16; ++c) {
+                uint32_t f[4];
+                ldmatrix_x4(k_tile + tile_unit<WIDTH>(key_row + n * 16, 2 * c + key_unit), f);
+                mma16816<BF16>(s[2 * n], q[c], f[0], f[1]);
+                mma16816<BF16>(s[2 * n + 1], q[c], f[2], f[3]);
+            }
+        // keys from this one on are behind a row's last
+        const int first_key = low + step * S::kStageKeys + key_warp * KEYS;
+        if (first_key + KEYS > min(min(limit[0], limit[1]), high)) {
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (first_key + n * 8 + 2 * t + (e & 1) >= min(limit[e >> 1], high)) s[n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float top = s[0][2 * half];
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
+            top = fmaxf(m[half], quad_max(top) * a.scale_log2);
+            const float base = top == -INFINITY ? 0.0f : top, shrink = ex2_approx_ftz(m[half] - base);
+            m[half] = top;
+            l[half] *= shrink;
+#pragma unroll
+            for (int c = 0; c < WIDTH / 8; ++c) o[c][2 * half] *= shrink, o[c][2 * half + 1] *= shrink;
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+                for (int e = 2 * half; e < 2 * half + 2; ++e) {
+                    s[n][e] = ex2_approx_ftz(__fmaf_rn(s[n][e], a.scale_log2, -base));
+                    l[half] += s[n][e];
+                }
+        }
+        const int value_row = key_warp * KEYS + ((lane >> 3) & 1) * 8 + (lane & 7), value_unit = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < KEYS / 16; ++n) {
+            const uint32_t p[4] = {pack16<BF16>(s[2 * n][0], s[2 * n][1]), pack16<BF16>(s[2 * n][2], s[2 * n][3]),
+                                   pack16<BF16>(s[2 * n + 1][0], s[2 * n + 1][1]), pack16<BF16>(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+            for (int c = 0; c < WIDTH / 16; ++c) {
+                uint32_t f[4];
+                ldmatrix_x4_trans(v_tile + tile_unit<WIDTH>(value_row + n * 16, 2 * c + value_unit), f);
+                mma16816<BF16>(o[2 * c], p, f[0], f[1]);
+                mma16816<BF16>(o[2 * c + 1], p, f[2], f[3]);
+            }
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // the stages are free
+#pragma unroll
+    for (int half = 0; half < 2; ++half) l[half] = quad_sum(l[half]);
+
+    if constexpr (KEY_WARPS > 1) {
+        float* sums = reinterpret_cast<float*>(smem);             // [KEY_WARPS][16][2]: m, l
+        float* tops = sums + KEY_WARPS * 16 * 2;                  // [KEY_WARPS][16][WIDTH]
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = g + 8 * half;
+            if (t == 0) sums[(warp * 16 + r) * 2] = m[half], sums[(warp * 16 + r) * 2 + 1] = l[half];
+#pragma unroll
+            for (int c = 0; c < WIDTH / 8; ++c)
+                *reinterpret_cast<float2*>(tops + (warp * 16 + r) * WIDTH + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
+        }
+        __syncthreads();
+        for (int r = warp; r < 16; r += KEY_WARPS) {  // a warp a row, lane i columns i, i + 32, ...
+            if (!live(r)) continue;
+            float top = -INFINITY, total = 0.0f, joined[WIDTH / 32] = {};
+#pragma unroll
+            for (int w = 0; w < KEY_WARPS; ++w) top = fmaxf(top, sums[(w * 16 + r) * 2]);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < KEY_WARPS; ++w) {
+                const float share = ex2_approx_ftz(sums[(w * 16 + r) * 2] - base);
+                total = __fmaf_rn(share, sums[(w * 16 + r) * 2 + 1], total);
+#pragma unroll
+                for (int i = 0; i < WIDTH / 32; ++i) joined[i] = __fmaf_rn(share, tops[(w * 16 + r) * WIDTH + lane + 32 * i], joined[i]);
+            }
+            bool finite = true;
+#pragma unroll
+            for (int i = 0; i < WIDTH / 32; ++i) finite = finite && isfinite(joined[i]);
+            const int token = token_of(r), head = head_of(r);
+            if (isfinite(total) && !__all_sync(0xffffffffu, finite)) {
+                recompute_row<BF16>(a, b, token, head, low, min(high, b.limit(token, a.causal)), split, lane);
+                continue;
+            }
+            const AttentionOut to = attention_out(a, split, b.row + token, head);
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int i = 0; i < WIDTH / 32; ++i) {
+                const int c = lane + 32 * i;
+                if (c >= a.width) continue;
+                if (a.splits > 1) to.part_out[c] = joined[i];
+                else to.out[c] = static_cast<uint16_t>(pack16<BF16>(joined[i] * inverse, 0.0f) & 0xffff);
+            }
+            if (a.splits > 1 && lane == 0) to.part_sums[0] = top, to.part_sums[1] = total;
+        }
+    } else {
+        uint8_t* staged = smem + warp * 16 * WIDTH * 2;
+        uint32_t again = 0;  // rows of the warp's 16 to compute again
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = row_warp * 16 + g + 8 * half;
+            bool finite = true;
+#pragma unroll
+            for (int c = 0; c < WIDTH / 8; ++c) finite = finite && isfinite(o[c][2 * half]) && isfinite(o[c][2 * half + 1]);
+            const uint32_t votes = __ballot_sync(0xffffffffu, !finite && isfinite(l[half]) && live(r));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((votes >> (4 * i)) & 15u) again |= 1u << (8 * half + i);
+            const float inverse = l[half] == 0.0f ? 0.0f : 1.0f / l[half];
+            if (a.splits > 1) {
+                if (live(r)) {
+                    const AttentionOut to = attention_out(a, split, b.row + token_of(r), head_of(r));
+#pragma unroll
+                    for (int c = 0; c < WIDTH / 8; ++c)
+                        if (c < units) *reinterpret_cast<float2*>(to.part_out + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
+                    if (t == 0) to.part_sums[0] = m[half], to.part_sums[1] = l[half];
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < WIDTH / 8; ++c)
+                    *reinterpret_cast<uint32_t*>(staged + tile_unit<WIDTH>(g + 8 * half, c) + 4 * t) =
+                        pack16<BF16>(o[c][2 * half] * inverse, o[c][2 * half + 1] * inverse);
+            }
+        }
+        __syncwarp();
+        if (a.splits == 1) {
+#pragma unroll
+            for (int i = 0; i < 16 * kUnits / 32; ++i) {
+                const int at = lane + i * 32, r = at / kUnits, unit = at % kUnits;
+                if (unit < units && live(row_warp * 16 + r))
+                    *reinterpret_cast<uint4*>(attention_out(a, 0, b.row + token_of(row_warp * 16 + r), head_of(row_warp * 16 + r)).out + unit * 8) =
+                        *reinterpret_cast<const uint4*>(staged + tile_unit<WIDTH>(r, unit));
+            }
+        }
+        __syncwarp();
+        for (; again != 0; again &= again - 1) {
+            const int r = row_warp * 16 + __ffs(again) - 1, token = token_of(r);
+            recompute_row<BF16>(a, b, token, head_of(r), low, min(high, b.limit(token, a.causal)), split, lane);
+        }
+    }
+}
+
+// Joins the splits of each (row, head), a warp each, in the order of the splits: with M the largest m,
+// out = sum 2^(m - M) o / sum 2^(m - M) l.
+template <bool BF16>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionArgs a) {
+    const int lane = threadIdx.x & 31;
+    grid_dependency_start();
+    const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads, at = blockIdx.x * 4ll + (threadIdx.x >> 5);
+    if (at >= count) return;
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_sums[(s * count + at) * 2]);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 sums = *reinterpret_cast<const float2*>(a.part_sums + (s * count + at) * 2);
+        if (sums.y == 0.0f) continue;  // a split without keys for this row
+        const float share = ex2_approx_ftz(sums.x - base);
+        total = __fmaf_rn(share, sums.y, total);
+        const float* part = a.part_out + (s * count + at) * a.width;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < a.width) o[i] = __fmaf_rn(share, part[lane + 32 * i], o[i]);
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < a.width) a.out[at * a.width + lane + 32 * i] = static_cast<uint16_t>(pack16<BF16>(o[i] * inverse, 0.0f) & 0xffff);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------
+
+namespace {
+
+template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
+cudaError_t launch_rows(AttentionArgs a, cudaStream_t stream) {
+    using S = RowsShape<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES>;
+    a.tile_heads = a.group < S::kRows ? a.group : S::kRows;
+    a.head_tiles = (a.group + a.tile_heads - 1) / a.tile_heads;
+    const int slots = a.lengths ? a.queries.count : packed_slots(a.queries.rows, S::kRows / a.tile_heads, a.queries.count);
+    auto kernel = attention_rows_kernel<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES, BF16>;
+    const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
+    if (status != cudaSuccess) return status;
+    return launch_dependent(kernel, dim3(slots, a.kv_heads * a.head_tiles, a.splits), dim3(S::kThreads), S::kSmemBytes, stream, a);
+}
+
+template <int WIDTH, bool BF16>
+cudaError_t launch_width(const AttentionArgs& a, bool few, cudaStream_t stream) {
+    return few ? launch_rows<WIDTH, 1, 4, 16, 3, BF16>(a, stream) : launch_rows<WIDTH, 4, 1, 64, 2, BF16>(a, stream);
+}
+
+template <bool BF16>
+cudaError_t launch_type(const AttentionArgs& a, bool few, cudaStream_t stream) {
+    const cudaError_t status = a.width <= 32   ? launch_width<32, BF16>(a, few, stream)
+                               : a.width <= 64 ? launch_width<64, BF16>(a, few, stream)
+                                               : launch_width<128, BF16>(a, few, stream);
+    if (status != cudaSuccess || a.splits == 1) return status;
+    const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads;
+    return launch_dependent(attention_join_kernel<BF16>, dim3(static_cast<unsigned>((count + 3) / 4)), dim3(128), 0, stream, a);
+}
+
+}  // namespace
+
+AttentionPlan attention_plan(const AttentionShape& s) {
+    AttentionPlan plan;
+    const int64_t sequences = s.sequences > 0 ? s.sequences : 1;
+    const int64_t mean_rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / sequences, mean_keys = s.cached ? s.capacity : s.key_rows / sequences;
+    plan.few = s.cached || mean_rows <= 16;
+    // blocks without a split, and how many fit a round of the 148 SMs twice over; a split keeps 256 keys or more
+    const int64_t group = s.heads / s.kv_heads, rows = plan.few ? 16 : 64, tile = rows / (group < rows ? group : rows);
+    const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
+    const int64_t wanted = 2 * 148 / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    const int64_t splits = wanted < most ? wanted : most;
+    plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
+    const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;
+    plan.workspace_bytes = plan.splits > 1 ? parts * (static_cast<size_t>(s.width) + 2) * sizeof(float) : 0;
+    return plan;
+}
+
+cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& x, float scale, void* workspace, cudaStream_t stream) {
+    const AttentionPlan plan = attention_plan(shape);
+    AttentionArgs a = {};
+    a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
+    a.q_row = x.q_row, a.q_head = x.q_head, a.k_row = x.k_row, a.k_head = x.k_head, a.v_row = x.v_row, a.v_head = x.v_head;
+    a.k_sequence = x.k_sequence, a.v_sequence = x.v_sequence;
+    a.heads = shape.heads, a.kv_heads = shape.kv_heads, a.width = shape.width, a.group = shape.heads / shape.kv_heads;
+    a.queries = PackedRows{x.q_offsets, shape.sequences, shape.q_rows};
+    a.k_offsets = x.k_offsets, a.k_rows = shape.key_rows;
+    a.lengths = x.lengths, a.capacity = shape.capacity;
+    a.causal = shape.causal;
+    a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+    a.splits = plan.splits;
+    a.part_sums = static_cast<float*>(workspace);
+    a.part_out = a.part_sums + static_cast<size_t>(plan.splits) * shape.q_rows * shape.heads * 2;
+    return shape.bf16 ? launch_type<true>(a, plan.few, stream) : launch_type<false>(a, plan.few, stream);
+}
+
+}  // namespace fry

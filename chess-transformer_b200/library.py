@@ -10,7 +10,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 LIBRARY_PATH = HERE / "libfry_b200.so"
 
-_c_int, _c_float, _ptr, _size = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_c_int, _c_i64, _c_float, _ptr, _size = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
 
 class FryError(RuntimeError):
@@ -58,6 +58,10 @@ SIGNATURES = {
     "fry_int8_matmul_i32": ([_ptr] * 3 + [_c_int] * 3 + [_ptr], _c_int),
     "fry_int8_matmul_scaled_bf16": ([_ptr] * 5 + [_c_int] * 3 + [_ptr], _c_int),
     "fry_attention_bf16": ([_ptr] * 4 + [_c_int] * 4 + [_ptr], _c_int),
+    "fry_packed_attention_workspace_bytes": ([_c_int] * 6, _size),
+    "fry_packed_attention": ([_ptr] * 6 + [_c_int] * 6 + [_c_i64] * 6 + [_c_float, _c_int, _c_int, _ptr, _size, _ptr], _c_int),
+    "fry_cached_attention_workspace_bytes": ([_c_int] * 5, _size),
+    "fry_cached_attention": ([_ptr] * 5 + [_c_int] * 5 + [_c_i64] * 8 + [_c_float, _c_int, _ptr, _size, _ptr], _c_int),
     "fry_norm_quant": ([_ptr, _ptr, _c_float, _ptr, _ptr, _c_int, _c_int, _ptr], _c_int),
     "fry_mix_norm_quant": ([_ptr] * 5 + [_c_float] + [_ptr] * 3 + [_c_int, _c_int, _ptr], _c_int),
     "fry_rotate_quant": ([_ptr] * 3 + [_c_int] * 3 + [_ptr], _c_int),

@@ -143,6 +143,131 @@ def _(q, k, v, heads):
     return torch.empty_like(q)
 
 
+def _call(function, index: int, *arguments) -> None:
+    """A library call on device `index` and its current stream, whatever device is current."""
+    arguments += (torch._C._cuda_getCurrentRawStream(index),)
+    if index == torch.cuda.current_device():
+        function(*arguments)
+    else:
+        with torch.cuda.device(index):
+            function(*arguments)
+
+
+def _direct(x: torch.Tensor, *others: torch.Tensor | None) -> bool:
+    """Whether a call may skip torch's dispatcher (about 12 us of a small call): not under torch.compile, which must see
+    the op, nor on fake tensors or where autograd would record it."""
+    if type(x) is not torch.Tensor or torch.compiler.is_compiling():
+        return False
+    return not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, *others))
+
+
+def _index32(name: str, tensor: torch.Tensor, what: str, count: int, device: torch.device) -> torch.Tensor:
+    if tensor.dtype != torch.int32 or tensor.dim() != 1 or tensor.shape[0] != count or tensor.device != device:
+        raise FryError(f"{name}: {what} must be int32 [{count}] on {device}, got {tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
+    return tensor.contiguous()
+
+
+def _strided(tensor: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
+    """A 16-bit tensor as the attention kernels read it, its last axis dense and its other strides and its start on 16
+    bytes (a copy if they are not), and those strides."""
+    strides = [s if n > 1 else 8 for s, n in zip(tensor.stride()[:-1], tensor.shape)]
+    if (tensor.stride(-1) != 1 and tensor.shape[-1] > 1) or any(s % 8 or not s for s in strides) or tensor.data_ptr() % 16:
+        tensor = tensor.clone(memory_format=torch.contiguous_format)
+        strides = [s if n > 1 else 8 for s, n in zip(tensor.stride()[:-1], tensor.shape)]
+    return tensor, strides
+
+
+def _attention_types(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    _cuda(name, q, k, v)
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise FryError(f"{name}: q, k and v must be of one type, fp16 or bf16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if k.device != q.device or v.device != q.device:
+        raise FryError(f"{name}: q, k and v must be on one device, got {q.device}, {k.device} and {v.device}")
+
+
+def _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale):
+    _attention_types("packed_attention", q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0:
+        raise FryError("packed_attention takes q [rows, heads, width] and k and v [key rows, kv_heads, width], heads a multiple of kv_heads, got "
+                       f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if q_offsets.dim() != 1 or q_offsets.shape[0] < 1:
+        raise FryError(f"packed_attention: q_offsets must be int32 [sequences + 1], got {q_offsets.dtype} {tuple(q_offsets.shape)}")
+    count = q_offsets.shape[0]
+    q_offsets = _index32("packed_attention", q_offsets, "q_offsets", count, q.device)
+    k_offsets = _index32("packed_attention", k_offsets, "k_offsets", count, q.device)
+    (q, (q_row, q_head)), (k, (k_row, k_head)), (v, (v_row, v_head)) = _strided(q), _strided(k), _strided(v)
+    (rows, heads, width), (key_rows, kv_heads, _) = q.shape, k.shape
+    out = q.new_empty(rows, heads, width)
+    lib = library()
+    size = lib.fry_packed_attention_workspace_bytes(rows, key_rows, count - 1, heads, kv_heads, width)
+    workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+    _call(lib.fry_packed_attention, q.device.index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
+          k_offsets.data_ptr(), rows, key_rows, count - 1, heads, kv_heads, width, q_row, q_head, k_row, k_head, v_row, v_head,
+          width ** -0.5 if scale is None else scale, causal, q.dtype == torch.bfloat16, workspace.data_ptr() if size else None, size)
+    return out
+
+
+@torch.library.custom_op("fry::packed_attention", mutates_args=())
+def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor, causal: bool,
+                         scale: float | None) -> torch.Tensor:
+    return _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale)
+
+
+@_packed_attention_op.register_fake
+def _(q, k, v, q_offsets, k_offsets, causal, scale):
+    return q.new_empty(q.shape)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor, causal: bool = True,
+                     scale: float | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over sequences packed one behind the other (the op fry::packed_attention): q [rows, heads,
+    width], k and v [key rows, kv_heads, width], fp16 or bf16, query head h on key/value head h // (heads // kv_heads);
+    sequence s has the rows q_offsets[s] to q_offsets[s + 1] and the keys k_offsets[s] to k_offsets[s + 1] (int32, on the
+    device). Causal, its queries are its last tokens: query i of nq sees keys j <= i + nk - nq. Rows that see no key, and
+    rows of no sequence, are 0. width a multiple of 8 up to 128; scale defaults to 1 / sqrt(width). No backward pass.
+    Strided views (of a projection's rows, say) are read in place where their last axis is dense and their other strides
+    are multiples of 8."""
+    run = _packed_attention if _direct(q, k, v) else torch.ops.fry.packed_attention
+    return run(q, k, v, q_offsets, k_offsets, causal, scale)
+
+
+def _cached_attention(q, k, v, lengths, scale):
+    _attention_types("cached_attention", q, k, v)
+    if (q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[2] or k.shape[2] == 0
+            or q.shape[1] % k.shape[2] != 0):
+        raise FryError("cached_attention takes q [sequences, heads, width] and k and v [sequences, capacity, kv_heads, width], heads a multiple of "
+                       f"kv_heads, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    lengths = _index32("cached_attention", lengths, "lengths", q.shape[0], q.device)
+    (q, (q_row, q_head)), (k, (k_sequence, k_row, k_head)), (v, (v_sequence, v_row, v_head)) = _strided(q), _strided(k), _strided(v)
+    (sequences, heads, width), (_, capacity, kv_heads, _) = q.shape, k.shape
+    out = q.new_empty(sequences, heads, width)
+    lib = library()
+    size = lib.fry_cached_attention_workspace_bytes(sequences, capacity, heads, kv_heads, width)
+    workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+    _call(lib.fry_cached_attention, q.device.index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(), sequences,
+          capacity, heads, kv_heads, width, q_row, q_head, k_sequence, k_row, k_head, v_sequence, v_row, v_head,
+          width ** -0.5 if scale is None else scale, q.dtype == torch.bfloat16, workspace.data_ptr() if size else None, size)
+    return out
+
+
+@torch.library.custom_op("fry::cached_attention", mutates_args=())
+def _cached_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float | None) -> torch.Tensor:
+    return _cached_attention(q, k, v, lengths, scale)
+
+
+@_cached_attention_op.register_fake
+def _(q, k, v, lengths, scale):
+    return q.new_empty(q.shape)
+
+
+def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float | None = None) -> torch.Tensor:
+    """packed_attention for one query token a sequence over a cache (the op fry::cached_attention): q [sequences, heads,
+    width], k and v [sequences, capacity, kv_heads, width] by any strides, of which sequence s has its first lengths[s] keys
+    (int32, on the device). What lies behind a length is not read; a length of 0 answers 0."""
+    run = _cached_attention if _direct(q, k, v) else torch.ops.fry.cached_attention
+    return run(q, k, v, lengths, scale)
+
+
 @torch.library.custom_op("fry::norm_quant", mutates_args=())
 def norm_quant(x: torch.Tensor, gain: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """`chess::norm_quant` (model/int8_blocks.py:191-193): int8 rows of RMSNorm(x) * gain and their scales."""

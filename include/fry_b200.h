@@ -36,8 +36,8 @@ const char* fry_version(void);
 
 /* Reads the current device's status word: *code 0 if no kernel recorded a fault, else the code (1 a bounded wait timed
  * out, 2 a board token outside the vocabulary, 3 a launch shape a kernel does not take, 4 misaligned shared memory, 5 a
- * lean lane's answer column outside the answer row, 6 a GPTQ Hessian that is not positive definite) and *where its
- * site. clear != 0 resets it. Synchronous. */
+ * lean lane's answer column outside the answer row, 6 a GPTQ Hessian that is not positive definite, 7 a request's
+ * offsets, length or adapter outside its tensors) and *where its site. clear != 0 resets it. Synchronous. */
 int fry_device_status(int* code, int* where, int clear);
 
 /* Every wait of a kernel on a barrier (a TMA load, a tensor-core commit, a cluster peer) is bounded: after the current
@@ -92,6 +92,34 @@ int fry_int8_matmul_scaled_bf16(const int8_t* x, const float* x_scale, const int
  * norms and no grouped heads. */
 int fry_attention_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, int B, int heads, int seq, int head_dim,
                        void* stream);
+
+/* Attention over packed sequences: out[t, h] = sum over the keys j that t sees of softmax(scale q[t, h] . k[j, g]) v[j, g],
+ * g = h / (heads / kv_heads), fp16 (bf16 == 0) or bf16 in and out, fp32 scores, sums and softmax. Sequence s has the query
+ * rows [q_offsets[s], q_offsets[s + 1]) of q [q_rows, heads, head_dim] and the key rows [k_offsets[s], k_offsets[s + 1])
+ * of k and v [k_rows, kv_heads, head_dim] (offsets int32 [sequences + 1], ascending, on the device). causal != 0: its
+ * queries are its last tokens, query i of nq sees keys j <= i + nk - nq of nk; else all nk. A row that sees no key, and a
+ * row of no sequence, answers 0. A key or value that a query does not see does not reach it, whatever it holds. Offsets
+ * outside their tensor or descending are read as the nearest row and recorded (code 7, where = the sequence); what the
+ * rows then hold is unspecified. out [q_rows, heads, head_dim] is dense and overlaps no input; strides are in elements,
+ * multiples of 8, the last axis dense; q, k, v and out 16-byte aligned. head_dim a multiple of 8 up to 128, heads a multiple of
+ * kv_heads up to 1024, scale positive. workspace: 16-byte aligned, of fry_packed_attention_workspace_bytes (0 where the
+ * keys are not split over blocks). Calls whose work overlaps on the GPU need workspaces of their own. The reference has
+ * no attention of this form: its template attention (model/fused_blocks.py:54-97) sees 70 tokens, all of them. */
+size_t fry_packed_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim);
+int fry_packed_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int32_t* q_offsets,
+                         const int32_t* k_offsets, int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim,
+                         int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                         int64_t v_head_stride, float scale, int causal, int bf16, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for one query token a sequence over a cache: q [sequences, heads, head_dim], k and v [sequences, capacity,
+ * kv_heads, head_dim] by their strides, of which sequence s has its first lengths[s] keys (int32 [sequences], on the
+ * device; one outside [0, capacity] is read as the nearest and recorded, code 7). What lies behind a length is not read. */
+size_t fry_cached_attention_workspace_bytes(int sequences, int capacity, int heads, int kv_heads, int head_dim);
+int fry_cached_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int32_t* lengths, int sequences,
+                         int capacity, int heads, int kv_heads, int head_dim, int64_t q_row_stride, int64_t q_head_stride,
+                         int64_t k_sequence_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_sequence_stride,
+                         int64_t v_row_stride, int64_t v_head_stride, float scale, int bf16, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* `chess::norm_quant` (model/int8_blocks.py:191-193, kernel :156-175): q[M, D] int8, scale[M] fp32 of
  * RMSNorm(x) * gain, a row's scale its absmax / 127. D a multiple of 8 up to 1024. */
