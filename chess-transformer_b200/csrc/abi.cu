@@ -80,6 +80,38 @@ int run_attention(const char* name, const fry::AttentionShape& shape, const fry:
     return check(fry::packed_attention(shape, x, scale, workspace, as_stream(stream)), name);
 }
 
+// Why the adapters' kernels do not take a shape ("" if they do).
+std::string adapter_refusal(int kind, int M, int N, int K, int requests, int adapters, int rank) {
+    const int k_unit = kind == 0 ? 16 : 8;
+    if (M < 0 || M > (1 << 24) || requests < 0 || requests > (1 << 24)) return "takes 0 to 2^24 rows and requests";
+    if (N <= 0 || N % 8 != 0 || K <= 0 || K % k_unit != 0)
+        return "takes N a multiple of 8 and K of " + std::to_string(k_unit) + ", got N " + std::to_string(N) + ", K " + std::to_string(K);
+    if (rank <= 0 || rank % 8 != 0 || rank > 128) return "takes a rank of a multiple of 8 up to 128 (pad smaller ones with zeros), got " + std::to_string(rank);
+    if (adapters <= 0 || static_cast<int64_t>(adapters) * N > 0x7fffff00) return "takes 1 or more adapters, their N columns together below 2^31";
+    return "";
+}
+
+size_t adapter_workspace_bytes(int kind, int M, int N, int requests, int rank) {
+    if (M <= 0 || !adapter_refusal(kind, M, N, 16, requests, 1, rank).empty()) return 0;
+    return fry::AdapterWorkspace(M, requests, rank, fry::adapter_tile_rows(kind, M, N)).total;
+}
+
+int run_adapters(const char* name, int kind, fry::GemmArgs& args, fry::AdapterArgs& p, const void* weight, int M, int N, int K, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+    std::string refusal = adapter_refusal(kind, M, N, K, p.requests, p.adapters, p.rank);
+    if (refusal.empty() && (!aligned16(p.x) || !aligned16(weight) || !aligned16(p.down) || !aligned16(p.up) || !aligned16(args.residual) ||
+                            !aligned16(args.out) || !aligned16(workspace)))
+        refusal = "needs 16-byte aligned x, weight, down, up, residual, out and workspace";
+    if (!refusal.empty()) return fail(FRY_ERROR_SHAPE, std::string(name) + " " + refusal);
+    if (M == 0) return check(cudaSuccess, "");
+    if (!p.x || !weight || !p.down || !p.up || !p.offsets || (p.requests > 0 && !p.ids) || !args.out)
+        return fail(FRY_ERROR_SHAPE, std::string(name) + " needs x, weight, down, up, offsets, ids and out");
+    if (!workspace || workspace_bytes < adapter_workspace_bytes(kind, M, N, p.requests, p.rank))
+        return fail(FRY_ERROR_SHAPE, std::string(name) + "'s workspace is smaller than " + name + "_workspace_bytes");
+    std::string detail;
+    return check(fry::adapter_linear(kind, args, p, weight, M, N, K, workspace, as_stream(stream), &detail), name, detail);
+}
+
 constexpr int kAnswerWidth = 1969;  // 1968 move logits, then the expected score
 constexpr uint64_t kMaxWaitLimitNs = 60000000000ull;  // the largest wait limit fry_set_wait_limit_ns takes: 60 s
 
@@ -342,6 +374,34 @@ int fry_attention_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
         return fail(FRY_ERROR_SHAPE, "fry_attention_bf16 needs 16-byte aligned q, k, v and out");
     std::string detail;
     return check(fry::attention64(q, k, v, out, B, heads, as_stream(stream), &detail), "fry_attention_bf16", detail);
+}
+
+size_t fry_int8_adapter_linear_workspace_bytes(int M, int N, int requests, int rank) { return adapter_workspace_bytes(0, M, N, requests, rank); }
+
+int fry_int8_adapter_linear(const int8_t* x, const float* x_scale, const int8_t* weight, const float* weight_scale, const uint16_t* bias,
+                            const uint16_t* residual, const uint16_t* down, const uint16_t* up, const int32_t* offsets, const int32_t* ids,
+                            uint16_t* out, int M, int N, int K, int requests, int adapters, int rank, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    fry::GemmArgs args;
+    args.x_scale = x_scale, args.w_scale = weight_scale, args.bias = bias, args.residual = residual, args.out = out;
+    fry::AdapterArgs p;
+    p.x = x, p.x_scale = x_scale, p.down = down, p.up = up, p.offsets = offsets, p.ids = ids;
+    p.requests = requests, p.adapters = adapters, p.rank = rank;
+    if (M > 0 && (!x_scale || !weight_scale)) return fail(FRY_ERROR_SHAPE, "fry_int8_adapter_linear needs both scales");
+    return run_adapters("fry_int8_adapter_linear", 0, args, p, weight, M, N, K, workspace, workspace_bytes, stream);
+}
+
+size_t fry_adapter_linear_workspace_bytes(int M, int N, int requests, int rank) { return adapter_workspace_bytes(1, M, N, requests, rank); }
+
+int fry_adapter_linear(const uint16_t* x, const uint16_t* weight, const uint16_t* bias, const uint16_t* residual, const uint16_t* down,
+                       const uint16_t* up, const int32_t* offsets, const int32_t* ids, uint16_t* out, int M, int N, int K, int requests,
+                       int adapters, int rank, void* workspace, size_t workspace_bytes, void* stream) {
+    fry::GemmArgs args;
+    args.bias = bias, args.residual = residual, args.out = out;
+    fry::AdapterArgs p;
+    p.x = x, p.down = down, p.up = up, p.offsets = offsets, p.ids = ids;
+    p.requests = requests, p.adapters = adapters, p.rank = rank;
+    return run_adapters("fry_adapter_linear", 1, args, p, weight, M, N, K, workspace, workspace_bytes, stream);
 }
 
 size_t fry_packed_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim) {

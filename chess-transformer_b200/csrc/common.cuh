@@ -17,6 +17,9 @@
 
 namespace fry {
 
+// The SMs of a B200, for choices that host code makes before a device is asked (workspace sizes among them).
+constexpr int kSms = 148;
+
 // Error codes a kernel records in the device-side status word (first failure wins).
 enum DeviceError : int {
     kOk = 0,

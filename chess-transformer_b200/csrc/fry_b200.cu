@@ -5,6 +5,7 @@
 #include "attention.cu"
 #include "attention64.cu"
 #include "packed_attention.cu"
+#include "adapters.cu"
 #include "heads.cu"
 #include "gptq.cu"
 #include "health.cu"

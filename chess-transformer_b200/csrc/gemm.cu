@@ -32,6 +32,7 @@
 // No TMA load multicasts.
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -59,13 +60,31 @@ constexpr int kNormedK = 768, kNormedSlices = kNormedK / kTileKBytes;  // the on
 constexpr int kMaxCluster = 4;  // kEpiLinearNorm: CTAs (column tiles) of a row block, one cluster
 constexpr int kNormBarrier = 2;  // named barrier of the 16 epilogue warps alone
 // fp16 linear epilogues (the bias and the residual optional)
-__host__ __device__ constexpr bool linear16(int epi) { return epi == kEpiLinearF16 || epi == kEpiLinearNorm || epi == kEpiMixF16; }
+__host__ __device__ constexpr bool linear16(int epi) {
+    return epi == kEpiLinearF16 || epi == kEpiLinearNorm || epi == kEpiMixF16 || epi == kEpiAdapterF16;
+}
+// epilogues of a linear with low-rank adapters
+__host__ __device__ constexpr bool adapts(int epi) { return epi == kEpiAdapterF16 || epi == kEpiAdapterInt8; }
+// epilogues whose residual may be absent
+__host__ __device__ constexpr bool optional_residual(int epi) { return linear16(epi) || epi == kEpiAdapterInt8; }
 // epilogues that mix the next block's input (residual and original row operands)
 __host__ __device__ constexpr bool mixes(int epi) { return epi == kEpiMix || epi == kEpiMixF16; }
 // int8 epilogues that scale the sums by the row's activation scale and the column's weight scale
-__host__ __device__ constexpr bool scaled(int epi) { return epi <= kEpiMix || epi == kEpiScaleBf16 || epi == kEpiBiasQkNorm; }
+__host__ __device__ constexpr bool scaled(int epi) { return epi <= kEpiMix || epi == kEpiScaleBf16 || epi == kEpiBiasQkNorm || epi == kEpiAdapterInt8; }
 // the bias epilogue, with or without the q/k norm after it
-__host__ __device__ constexpr bool biased(int epi) { return epi == kEpiBias || epi == kEpiBiasQkNorm; }
+__host__ __device__ constexpr bool biased(int epi) { return epi == kEpiBias || epi == kEpiBiasQkNorm || epi == kEpiAdapterInt8; }
+
+// A linear with adapters gets theirs with its arguments: the maps of low [slots * tile rows, rank] and of up
+// [adapters * N, rank], boxes of 64 columns (zeros past the rank) by the A and B operands' rows.
+struct AdapterGemmArgs : GemmArgs {
+    CUtensorMap map_low, map_up;
+    AdapterArgs adapters;
+    const uint16_t* weight;  // fp16 [N, K]
+    int slots, M, N, K;
+};
+template <int EPI>
+using ArgsOf = std::conditional_t<adapts(EPI), AdapterGemmArgs, GemmArgs>;
+constexpr int kRankStep = 64;  // rank columns a pipeline stage holds: 128 bytes of fp16
 
 // SUB: the columns an epilogue sub-tile stages (whole 64-column boxes, dividing BN); a BN-wide accumulator (one MMA of
 // up to N = 256) leaves in BN / SUB sub-tiles, so the staging slots stay small beside the pipeline stages.
@@ -88,7 +107,7 @@ struct GemmShape {
     // fp16 outputs are staged for TMA stores; int32 and fp32 outputs are stored by their threads
     static constexpr bool kStaged = EPI != kEpiInt32 && EPI != kEpiLinearF32;
     // the epilogue's row operands (residual, and original when mixing), loaded into the staging slots
-    static constexpr int kRowTensors = mixes(EPI) ? 2 : (EPI == kEpiResidual || linear16(EPI)) ? 1 : 0;
+    static constexpr int kRowTensors = mixes(EPI) ? 2 : (EPI == kEpiResidual || optional_residual(EPI)) ? 1 : 0;
     // chunks of 16 columns a thread takes in a sub-tile (the 4 warps of a TMEM lane quarter share a sub-tile's chunks)
     static constexpr int kChunksPerSub = SUB / (kChunkCols * kChunkParts) > 0 ? SUB / (kChunkCols * kChunkParts) : 1;
     static constexpr int kSubs = BN / SUB;       // sub-tiles a tile
@@ -118,7 +137,9 @@ struct GemmShape {
     static constexpr int kStagesFit = (kSmemBudget - kResidentBytes - kRowScaleBytes - kIoBytes - kColumnBytes - kNormBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static_assert(kStages >= 2, "at least two pipeline stages");
-    static constexpr int kAccCols = BN * (GATED ? 2 : 1);  // one accumulator; two are allocated
+    // the adapters' fp32 sums beside int8's int32 sums take a second half of the accumulator
+    static constexpr int kMmaCols = BN * (GATED ? 2 : 1);
+    static constexpr int kAccCols = kMmaCols * (EPI == kEpiAdapterInt8 ? 2 : 1);  // one accumulator; two are allocated
     static constexpr int kTmemCols = 2 * kAccCols <= 64 ? 64 : 2 * kAccCols <= 128 ? 128 : 2 * kAccCols <= 256 ? 256 : 512;
     static_assert(2 * kAccCols <= 512, "two accumulators fit TMEM's 512 columns");
     static constexpr int kSmemBytes =
@@ -324,13 +345,57 @@ FRY_DEVICE void normalize_qk(const GemmArgs& p, int column, const float* gains, 
     else normalize_qk24(p, key, column % 48, gains, near, result);
 }
 
+// A row tile's slots [x, y). With offsets that descend a tile's may not have been written: none then, or some in range.
+FRY_DEVICE int2 adapter_slots(const AdapterGemmArgs& p, int row_tile) {
+    const int2 slots = p.adapters.tile_slots[row_tile];
+    return slots.x >= 0 && slots.y <= p.slots ? slots : make_int2(0, 0);
+}
+
+// The sums of element (m, n) from its own request's adapter alone (kEpiAdapterF16: with x . weight). A tile's adapter steps
+// multiply the rows of other requests by zeros, so an adapter that is not finite makes them NaN: elements that are not
+// finite are summed again this way, whatever made them so. Slow, and seldom run.
+template <int EPI>
+__device__ __noinline__ float adapter_sums(const AdapterGemmArgs& p, int m, int n) {
+    float sum = 0.0f;
+    if constexpr (EPI == kEpiAdapterF16) {
+        const uint16_t* x = static_cast<const uint16_t*>(p.adapters.x) + static_cast<size_t>(m) * p.K;
+        const uint16_t* w = p.weight + static_cast<size_t>(n) * p.K;
+        for (int k = 0; k < p.K; ++k) sum = __fmaf_rn(h2f_bits(x[k]), h2f_bits(w[k]), sum);
+    }
+    const int tile = m / p.adapters.tile_rows, rank = p.adapters.rank;
+    const int2 slots = adapter_slots(p, tile);
+    for (int slot = slots.x; slot < slots.y; ++slot) {
+        const int adapter = p.adapters.slot_adapter[slot], request = slot - tile - 1;
+        if (adapter < 0 || adapter >= p.adapters.adapters || request < 0 || request >= p.adapters.requests) continue;
+        if (m < p.adapters.offsets[request] || m >= p.adapters.offsets[request + 1]) continue;
+        const uint16_t* low = p.adapters.low + (static_cast<size_t>(slot) * p.adapters.tile_rows + m % p.adapters.tile_rows) * rank;
+        const uint16_t* up = p.adapters.up + (static_cast<size_t>(adapter) * p.N + n) * rank;
+        for (int j = 0; j < rank; ++j) sum = __fmaf_rn(h2f_bits(low[j]), h2f_bits(up[j]), sum);
+    }
+    return sum;
+}
+// A row's 16 sums from `column` on, those that are not finite summed again (rows and columns of the output alone).
+template <int EPI>
+FRY_DEVICE void finite_sums(const AdapterGemmArgs& p, size_t row, int column, uint32_t (&sums)[16]) {
+    uint64_t zero2 = pair2(0.0f, 0.0f);  // 0 * sum is 0 where the sum is finite, else NaN
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) zero2 = fma2(pair2(__uint_as_float(sums[e]), __uint_as_float(sums[e + 1])), pair2(0.0f, 0.0f), zero2);
+    const float2 zero = lanes(zero2);
+    if (zero.x + zero.y == 0.0f) return;
+    const int m = static_cast<int>((row - column) / p.N);
+    if (m >= p.M) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (column + e < p.N && !isfinite(__uint_as_float(sums[e]))) sums[e] = __float_as_uint(adapter_sums<EPI>(p, m, column + e));
+}
+
 // Applies the epilogue to one row's 16 consecutive columns. acc (and up, gated) hold the raw TMEM words, xs the row's
 // activation scale, rs and is the next block's input-mix scales, scale and second the chunk's column operands in shared
 // memory. Staged epilogues read the row's residual (and original) from its staged chunk and write the fp16 results over
 // it (and into result, as fp16 pairs); int32 and fp32 epilogues store [n, n + valid) of row index `row` directly.
 // gains and near: the q/k norm's column gains and, at dq 24, the fp16 outputs of the chunks beside this one.
 template <int EPI>
-FRY_DEVICE void epilogue16(const GemmArgs& p, float xs, float rs, float is, const uint32_t (&acc)[16], const uint32_t (&up)[16],
+FRY_DEVICE void epilogue16(const ArgsOf<EPI>& p, float xs, float rs, float is, uint32_t (&acc)[16], uint32_t (&up)[16],
                            const float* scale, const float* second, const StagedChunk& staged, const StagedChunk& original, size_t row,
                            int valid, int column, const float* gains, const uint32_t (&near)[2][8], uint32_t (&result)[8]) {
     if constexpr (EPI == kEpiInt32) {
@@ -352,10 +417,12 @@ FRY_DEVICE void epilogue16(const GemmArgs& p, float xs, float rs, float is, cons
             }
         return;
     } else {
-        constexpr bool kResidual = EPI == kEpiResidual || mixes(EPI) || linear16(EPI);
+        if constexpr (EPI == kEpiAdapterF16) finite_sums<EPI>(p, row, column, acc);
+        if constexpr (EPI == kEpiAdapterInt8) finite_sums<EPI>(p, row, column, up);
+        constexpr bool kResidual = EPI == kEpiResidual || mixes(EPI) || optional_residual(EPI);
         uint4 residual_words[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, original_words[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if constexpr (kResidual) {
-            if (!linear16(EPI) || p.residual != nullptr) residual_words[0] = *staged.at(0), residual_words[1] = *staged.at(1);
+            if (!optional_residual(EPI) || p.residual != nullptr) residual_words[0] = *staged.at(0), residual_words[1] = *staged.at(1);
         }
         if constexpr (mixes(EPI)) original_words[0] = *original.at(0), original_words[1] = *original.at(1);
         const uint16_t* res = reinterpret_cast<const uint16_t*>(residual_words);
@@ -387,6 +454,10 @@ FRY_DEVICE void epilogue16(const GemmArgs& p, float xs, float rs, float is, cons
             uint64_t value2;
             if constexpr (biased(EPI)) {
                 value2 = fma2(mul2(acc2, xs2), scale2, second2);
+                if constexpr (EPI == kEpiAdapterInt8) {  // up: the adapters' fp32 sums
+                    value2 = add2(value2, pair2(__uint_as_float(up[e]), __uint_as_float(up[e + 1])));
+                    if (p.residual) value2 = add2(value2, pair2(h2f_exact(res[e]), h2f_exact(res[e + 1])));
+                }
             } else if constexpr (EPI == kEpiScaleBf16) {
                 value2 = mul2(mul2(acc2, xs2), scale2);
             } else if constexpr (EPI == kEpiGated || EPI == kEpiGatedF16) {
@@ -541,11 +612,28 @@ FRY_DEVICE void norm_rows_of_tile(const GemmArgs& p, float* norm_smem, uint64_t*
     }
 }
 
+// A row tile's adapter steps, step(slot, adapter, first rank column) for each in order until one returns false: its
+// requests' slots that have an adapter, kRankStep columns of the rank a step. int8's fp32 sums need one to start them, so
+// a tile without adapters takes a step that lies behind both tensors (zeros).
+template <int EPI, typename Step>
+FRY_DEVICE bool adapter_steps(const AdapterGemmArgs& p, int row_tile, Step step) {
+    const int2 slots = adapter_slots(p, row_tile);
+    bool any = false;
+    for (int slot = slots.x; slot < slots.y; ++slot) {
+        const int adapter = p.adapters.slot_adapter[slot];
+        if (adapter < 0 || adapter >= p.adapters.adapters) continue;
+        any = true;
+        for (int column = 0; column < p.adapters.rank; column += kRankStep)
+            if (!step(slot, adapter, column)) return false;
+    }
+    return any || EPI != kEpiAdapterInt8 || step(p.slots, p.adapters.adapters, 0);
+}
+
 template <int KIND, int BN, bool GATED, int EPI, int SUB, int NKS, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_residual,
-                const __grid_constant__ CUtensorMap map_original, const GemmArgs args, int M, int N, int K) {
+                const __grid_constant__ CUtensorMap map_original, const __grid_constant__ ArgsOf<EPI> args, int M, int N, int K) {
     using S = GemmShape<KIND, BN, GATED, EPI, SUB, NKS, PAIR>;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_addr(smem) & 1023u) {  // uniform across the CTA: every thread leaves before any barrier
@@ -673,7 +761,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
         }
     }
-    grid_dependency_start();  // setup done: now the operands of earlier kernels
+    // setup done: now the operands of earlier kernels. With adapters the kernel before this one reads x and writes low, and
+    // it started only after those before it were done, so x, the weights and the residual may be read at once; the
+    // producer and the MMA warp wait for low where a tile first needs it.
+    if constexpr (!adapts(EPI)) grid_dependency_start();
 
     if (warp == kProducerWarp) {
         if (elect_one()) {
@@ -697,6 +788,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     }
                     if constexpr (NKS == 0) load_a(a, s, kt, m0);
                 }
+                if constexpr (adapts(EPI)) {
+                    if (tile == first_tile) grid_dependency_start();
+                    ok = ok && adapter_steps<EPI>(args, tile / n_blocks, [&](int slot, int adapter, int column) {
+                        const int s = it % S::kStages;
+                        if (!mbar_wait(&empty[s], ((it++ / S::kStages) & 1) ^ 1, 10)) return false;
+                        arm_stage(s);
+                        uint8_t* a = stages + s * S::kStageBytes;
+                        const int low_row = slot * kTileRows + rank * kBlockM, up_row = adapter * N + n0 + rank * (PAIR ? S::kBRows : 0);
+                        if constexpr (PAIR) {
+                            tma_load_2d_pair(a, &args.map_low, peer_smem(&full[s], 0), column, low_row);
+                            tma_load_2d_pair(a + S::kABytes, &args.map_up, peer_smem(&full[s], 0), column, up_row);
+                        } else {
+                            tma_load_2d(a, &args.map_low, &full[s], column, low_row);
+                            tma_load_2d(a + S::kABytes, &args.map_up, &full[s], column, up_row);
+                        }
+                        return true;
+                    });
+                }
             }
         }
     } else if (warp == kMmaWarp) {
@@ -712,7 +821,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if ((!PAIR || rank == 0) && elect_one()) {
             // gated: the gate's and the up's B boxes lie back to back, 2 BN rows at the swizzle's 1024 bytes per 8, so one MMA of
             // N = 2 BN fills both accumulator halves
-            constexpr uint32_t idesc = instr_desc<KIND>(S::kAccCols, kTileRows);
+            constexpr uint32_t idesc = instr_desc<KIND>(S::kMmaCols, kTileRows);
             int it = 0, local = 0, units = 0;
             bool ok = true;
             for (int tile = first_tile; tile < tiles && ok; tile = next_tile(tile), ++local) {
@@ -741,6 +850,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     }
                     commit(&empty[s]);
                 }
+                if constexpr (adapts(EPI)) {
+                    if (tile == first_tile) grid_dependency_start();
+                    // int8: the adapters' sums are fp32, in the accumulator's second half, which the first step starts
+                    constexpr uint32_t adapter_idesc = instr_desc<1>(BN, kTileRows);
+                    const uint32_t sums = accumulator + (KIND == 0 ? BN : 0);
+                    uint32_t accumulate = KIND == 0 ? 0u : 1u;
+                    ok = ok && adapter_steps<EPI>(args, tile / n_blocks, [&](int, int, int column) {
+                        const int s = it % S::kStages;
+                        if (!mbar_wait(&full[s], (it++ / S::kStages) & 1, 12)) return false;
+                        tc_fence_after();
+                        const uint32_t a = smem_addr(stages + s * S::kStageBytes), b = a + S::kABytes;
+                        const int count = (min(kRankStep, args.adapters.rank - column) + 15) / 16;
+                        for (int k = 0; k < count; ++k, accumulate = 1u) {
+                            const uint64_t da = smem_desc_sw128(a + k * kMmaKBytes), db = smem_desc_sw128(b + k * kMmaKBytes);
+                            if constexpr (PAIR) mma_ss_pair<1>(sums, da, db, adapter_idesc, accumulate);
+                            else mma_ss<1>(sums, da, db, adapter_idesc, accumulate);
+                        }
+                        commit(&empty[s]);
+                        return true;
+                    });
+                }
                 commit(&tmem_full[buffer]);
             }
         }
@@ -751,7 +881,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // reads are done: with row operands it waits for them here, before loading the rows; without, it waits for all
         // but the last kSlots - 2 groups, so sub-tile j's stores keep reading while the next kSlots - 2 sub-tiles stage.
         if constexpr (S::kStaged) {
-            const bool has_rows = S::kRowTensors > 0 && (!linear16(EPI) || args.residual != nullptr);
+            const bool has_rows = S::kRowTensors > 0 && (!optional_residual(EPI) || args.residual != nullptr);
             const bool issuer = lane == 0;
             auto load_rows = [&](int tile, int sub, int slot) {
                 if (!issuer || !has_rows || tile >= tiles) return;
@@ -798,7 +928,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             rs = h2f_bits(*args.residual_scale);
             is = h2f_bits(*args.input_scale);
         }
-        const bool has_rows = S::kRowTensors > 0 && (!linear16(EPI) || args.residual != nullptr);
+        const bool has_rows = S::kRowTensors > 0 && (!optional_residual(EPI) || args.residual != nullptr);
         auto tile_origin = [&](int tile, int& m0, int& n0) {
             m0 = row0(tile);
             n0 = column0(tile);
@@ -890,7 +1020,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         }
                         uint32_t acc[16], up[16];
                         tmem_load16(lane_base + c, acc);
-                        if constexpr (GATED) tmem_load16(lane_base + BN + c, up);
+                        if constexpr (GATED || EPI == kEpiAdapterInt8) tmem_load16(lane_base + BN + c, up);
                         tmem_load_wait();
                         const int c_sub = c - sub * SUB;
                         const int box = c_sub / kBoxCols, unit = 2 * ((c_sub % kBoxCols) / kChunkCols), swizzle = row_in_tile & 7;
@@ -1007,7 +1137,7 @@ bool make_box_map(CUtensorMap* map, const void* base, int cols, int rows, std::s
 }
 
 template <int KIND, int BN, bool GATED, int EPI, int SUB = BN, int NKS = 0, bool PAIR = false>
-cudaError_t launch(const void* a, const void* b, const GemmArgs& args, int M, int N, int K, cudaStream_t stream, std::string* error) {
+cudaError_t launch(const void* a, const void* b, const ArgsOf<EPI>& args, int M, int N, int K, cudaStream_t stream, std::string* error) {
     using S = GemmShape<KIND, BN, GATED, EPI, SUB, NKS, PAIR>;
     auto kernel = gemm_kernel<KIND, BN, GATED, EPI, SUB, NKS, PAIR>;
     const cudaError_t attribute = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
@@ -1070,6 +1200,22 @@ cudaError_t launch(const void* a, const void* b, const GemmArgs& args, int M, in
     }
     return launch_dependent(kernel, dim3(grid), dim3(kGemmThreads), S::kSmemBytes, stream, map_a, map_b, map_out, map_residual,
                             map_original, args, M, N, K);
+}
+
+// A linear with adapters: their maps, then launch().
+template <int KIND, int BN, int EPI, bool PAIR>
+cudaError_t launch_adapters(const AdapterArgs& adapters, const void* weight, const GemmArgs& args, int slots, int M, int N, int K,
+                            cudaStream_t stream, std::string* error) {
+    using S = GemmShape<KIND, BN, false, EPI, 64, 0, PAIR>;
+    AdapterGemmArgs all;
+    static_cast<GemmArgs&>(all) = args;
+    all.adapters = adapters;
+    all.weight = static_cast<const uint16_t*>(weight);
+    all.slots = slots, all.M = M, all.N = N, all.K = K;
+    if (!make_map(&all.map_low, adapters.low, 2, adapters.rank, slots * adapters.tile_rows, kBlockM, error) ||
+        !make_map(&all.map_up, adapters.up, 2, adapters.rank, adapters.adapters * N, S::kBRows, error))
+        return cudaErrorInvalidValue;
+    return launch<KIND, BN, false, EPI, 64, 0, PAIR>(adapters.x, weight, all, M, N, K, stream, error);
 }
 
 }  // namespace
@@ -1195,6 +1341,31 @@ cudaError_t gemm(int kind, int epilogue, const void* a, const void* b, const Gem
     }
     if (error) *error = "no GEMM for this kind and epilogue";
     return cudaErrorInvalidValue;
+}
+
+namespace {
+
+// The widest tile whose count fills the SMs, as gemm() chooses it; int8 keeps two fp32 halves of 128 columns in TMEM.
+int adapter_tile_columns(int kind, int M, int N) {
+    const int row_blocks = (M + kBlockM - 1) / kBlockM;
+    auto tiles = [&](int bn) { return row_blocks * ((N + bn - 1) / bn); };
+    if (kind == 1 && tiles(256) >= kSms) return 256;
+    return tiles(128) >= kSms ? 128 : 64;
+}
+
+}  // namespace
+
+int adapter_tile_rows(int kind, int M, int N) { return kind == 1 && adapter_tile_columns(kind, M, N) == 256 ? 2 * kBlockM : kBlockM; }
+
+cudaError_t adapter_gemm(int kind, const AdapterArgs& adapters, const void* weight, const GemmArgs& args, int slots, int M, int N, int K,
+                         cudaStream_t stream, std::string* error) {
+    const int columns = adapter_tile_columns(kind, M, N);
+    if (kind == 0)
+        return columns == 128 ? launch_adapters<0, 128, kEpiAdapterInt8, false>(adapters, weight, args, slots, M, N, K, stream, error)
+                              : launch_adapters<0, 64, kEpiAdapterInt8, false>(adapters, weight, args, slots, M, N, K, stream, error);
+    if (columns == 256) return launch_adapters<1, 256, kEpiAdapterF16, true>(adapters, weight, args, slots, M, N, K, stream, error);
+    if (columns == 128) return launch_adapters<1, 128, kEpiAdapterF16, false>(adapters, weight, args, slots, M, N, K, stream, error);
+    return launch_adapters<1, 64, kEpiAdapterF16, false>(adapters, weight, args, slots, M, N, K, stream, error);
 }
 
 }  // namespace fry

@@ -25,6 +25,8 @@ enum GemmEpilogue : int {
     kEpiMixF16 = 9,     // fp16: (acc + bias) + residual rounded to fp16, then fp16(fma(stream, rs, original * is))
     kEpiScaleBf16 = 10, // int8: bf16((acc * xs) * ws), the scaled GEMM of the isolated-kernel benchmark (no reference op)
     kEpiBiasQkNorm = 11,// int8: kEpiBias, then the attention's q and k RMSNorm with gains on the query and key columns (qk_*)
+    kEpiAdapterF16 = 12,   // fp16: as kEpiLinearF16, the sums with the requests' low-rank adapters in them
+    kEpiAdapterInt8 = 13,  // int8: fp16((fma(acc * xs, ws, bias) + the adapters' fp32 sums) + residual), residual optional
 };
 
 struct GemmArgs {
@@ -58,6 +60,34 @@ struct GemmArgs {
 // kind 0: int8 A [M, K], B [N, K] (gated: [2N, K]); kind 1: fp16 A [M, K], B [N, K].
 cudaError_t gemm(int kind, int epilogue, const void* a, const void* b, const GemmArgs& args, int M, int N, int K, cudaStream_t stream,
                  std::string* error);
+
+// Low-rank adapters beside a linear (adapters.cu; the GEMM's part in gemm.cu): request s has the rows [offsets[s],
+// offsets[s + 1]) and the adapter ids[s] (-1: none), down [adapters, rank, K] and up [adapters, N, rank] fp16.
+struct AdapterArgs {
+    const void* x = nullptr;               // int8 or fp16 [M, K]
+    const float* x_scale = nullptr;        // int8: [M]
+    const uint16_t* down = nullptr;
+    const uint16_t* up = nullptr;
+    const int32_t* offsets = nullptr;      // [requests + 1]
+    const int32_t* ids = nullptr;          // [requests]
+    int requests = 0, adapters = 0, rank = 0;
+    int tile_rows = 0;                     // the GEMM's row tile
+    // in the workspace: x down^T of each slot's tile (rows of other requests 0) fp16 [slots, tile_rows, rank], a tile's
+    // slots [first, last), and a slot's adapter (-1: none)
+    uint16_t* low = nullptr;
+    int2* tile_slots = nullptr;
+    int32_t* slot_adapter = nullptr;
+};
+struct AdapterWorkspace {
+    size_t slots, tile_slots, slot_adapter, total;
+    AdapterWorkspace(int M, int requests, int rank, int tile_rows);
+};
+int adapter_tile_rows(int kind, int M, int N);
+cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& adapters, const void* weight, int M, int N, int K, void* workspace,
+                           cudaStream_t stream, std::string* error);
+// gemm() with the adapters' steps (kind 0: kEpiAdapterInt8, 1: kEpiAdapterF16), after the kernel that made low
+cudaError_t adapter_gemm(int kind, const AdapterArgs& adapters, const void* weight, const GemmArgs& args, int slots, int M, int N, int K,
+                         cudaStream_t stream, std::string* error);
 
 // Row kernels (rows.cu).
 cudaError_t norm_quant(const uint16_t* x, const uint16_t* original, const uint16_t* residual_scale, const uint16_t* input_scale,

@@ -484,10 +484,10 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     const int64_t sequences = s.sequences > 0 ? s.sequences : 1;
     const int64_t mean_rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / sequences, mean_keys = s.cached ? s.capacity : s.key_rows / sequences;
     plan.few = s.cached || mean_rows <= 16;
-    // blocks without a split, and how many fit a round of the 148 SMs twice over; a split keeps 256 keys or more
+    // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
     const int64_t group = s.heads / s.kv_heads, rows = plan.few ? 16 : 64, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
-    const int64_t wanted = 2 * 148 / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    const int64_t wanted = 2 * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
     const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;

@@ -55,6 +55,10 @@ SIGNATURES = {
     "fry_wait_probe": ([_ptr], _c_int),
     "fry_int8_linear": ([_ptr] * 10 + [_c_int] * 4 + [_ptr], _c_int),
     "fry_int8_linear_normed": ([_ptr, _ptr, _c_float] + [_ptr] * 4 + [_c_int] * 4 + [_ptr], _c_int),
+    "fry_int8_adapter_linear_workspace_bytes": ([_c_int] * 4, _size),
+    "fry_int8_adapter_linear": ([_ptr] * 11 + [_c_int] * 6 + [_ptr, _size, _ptr], _c_int),
+    "fry_adapter_linear_workspace_bytes": ([_c_int] * 4, _size),
+    "fry_adapter_linear": ([_ptr] * 9 + [_c_int] * 6 + [_ptr, _size, _ptr], _c_int),
     "fry_int8_matmul_i32": ([_ptr] * 3 + [_c_int] * 3 + [_ptr], _c_int),
     "fry_int8_matmul_scaled_bf16": ([_ptr] * 5 + [_c_int] * 3 + [_ptr], _c_int),
     "fry_attention_bf16": ([_ptr] * 4 + [_c_int] * 4 + [_ptr], _c_int),

@@ -268,6 +268,114 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     return run(q, k, v, lengths, scale)
 
 
+def _aligned(tensor: torch.Tensor) -> torch.Tensor:
+    """Dense rows that start on 16 bytes (a copy if they do not)."""
+    tensor = tensor.contiguous()
+    return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
+
+
+def _adapter_shapes(name: str, x, weight, bias, residual, down, up, offsets, ids) -> tuple[int, int, int, int, int, int]:
+    """(M, N, K, requests, adapters, rank) of a linear with adapters, or FryError."""
+    for tensor in (weight, bias, residual, down, up, offsets, ids):
+        if tensor is not None and tensor.device != x.device:
+            raise FryError(f"{name}: x is on {x.device}, another operand on {tensor.device}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise FryError(f"{name} takes x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != K or up.shape[1] != N or up.shape[0] != down.shape[0] or up.shape[2] != down.shape[1]:
+        raise FryError(f"{name} takes down [adapters, rank, {K}] and up [adapters, {N}, rank], got {tuple(down.shape)} and {tuple(up.shape)}")
+    for tensor, what in ((bias, "bias"), (residual, "residual"), (down, "down"), (up, "up")):
+        _dtype(name, tensor, torch.float16, what)
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise FryError(f"{name}: bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
+        raise FryError(f"{name}: residual must be {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+    requests = ids.shape[0] if ids.dim() == 1 else -1
+    _index32(name, ids, "ids", requests, x.device)
+    _index32(name, offsets, "offsets", requests + 1, x.device)
+    return x.numel() // K, N, K, requests, down.shape[0], down.shape[1]
+
+
+def _adapter_call(x, out, shapes, function, size, *operands):
+    """The library call of a linear with adapters into `out`: its operands' pointers, `out`, the sizes and a workspace."""
+    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
+    _call(function, x.device.index, *(None if t is None else t.data_ptr() for t in operands), out.data_ptr(), *shapes, workspace.data_ptr(), size)
+    return out
+
+
+def _adapter_linear(x, weight, bias, residual, down, up, offsets, ids):
+    _cuda("adapter_linear", x)
+    _dtype("adapter_linear", x, torch.float16, "x")
+    _dtype("adapter_linear", weight, torch.float16, "weight")
+    shapes = _adapter_shapes("adapter_linear", x, weight, bias, residual, down, up, offsets, ids)
+    M, N, _, requests, _, rank = shapes
+    lib = library()
+    return _adapter_call(x, x.new_empty(*x.shape[:-1], N), shapes, lib.fry_adapter_linear, lib.fry_adapter_linear_workspace_bytes(M, N, requests, rank),
+                         _aligned(x), _aligned(weight), bias.contiguous() if bias is not None else None,
+                         _aligned(residual) if residual is not None else None, _aligned(down), _aligned(up), offsets.contiguous(), ids.contiguous())
+
+
+@torch.library.custom_op("fry::adapter_linear", mutates_args=())
+def _adapter_linear_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None, down: torch.Tensor,
+                       up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    return _adapter_linear(x, weight, bias, residual, down, up, offsets, ids)
+
+
+@_adapter_linear_op.register_fake
+def _(x, weight, bias, residual, down, up, offsets, ids):
+    return x.new_empty(*x.shape[:-1], weight.shape[0])
+
+
+def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None, down: torch.Tensor,
+                   up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """A linear with a low-rank adapter for each request's rows (the op fry::adapter_linear), fp16:
+    x W^T + bias + residual, plus (x down[a]^T) up[a]^T for the rows offsets[s] to offsets[s + 1] of request s, a = ids[s].
+    x [..., K], weight [N, K] as nn.Linear holds it, down [adapters, rank, K], up [adapters, N, rank]; offsets [requests + 1]
+    and ids [requests] int32 on the device; rows of no request and those of ids -1 have no adapter. rank a multiple of 8 up
+    to 128 (pad smaller ones with zeros), N and K multiples of 8. No backward pass."""
+    run = _adapter_linear if _direct(x, weight, bias, residual, down, up) else torch.ops.fry.adapter_linear
+    return run(x, weight, bias, residual, down, up, offsets, ids)
+
+
+def _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids):
+    name = "int8_adapter_linear"
+    _cuda(name, x, x_scale, weight_scale)
+    _dtype(name, x, torch.int8, "x")
+    _dtype(name, weight, torch.int8, "weight")
+    shapes = _adapter_shapes(name, x, weight, bias, residual, down, up, offsets, ids)
+    M, N, _, requests, _, rank = shapes
+    _dtype(name, x_scale, torch.float32, "x_scale")
+    _dtype(name, weight_scale, torch.float32, "weight_scale")
+    if x_scale.numel() != M or weight_scale.numel() != N or x_scale.device != x.device or weight_scale.device != x.device:
+        raise FryError(f"{name} takes a scale a row of x and of weight on {x.device}, got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
+    lib = library()
+    out = x.new_empty(*x.shape[:-1], N, dtype=torch.float16)
+    return _adapter_call(x, out, shapes, lib.fry_int8_adapter_linear, lib.fry_int8_adapter_linear_workspace_bytes(M, N, requests, rank), _aligned(x),
+                         x_scale.contiguous(), _aligned(weight), weight_scale.contiguous(), bias.contiguous() if bias is not None else None,
+                         _aligned(residual) if residual is not None else None, _aligned(down), _aligned(up), offsets.contiguous(), ids.contiguous())
+
+
+@torch.library.custom_op("fry::int8_adapter_linear", mutates_args=())
+def _int8_adapter_linear_op(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None,
+                            residual: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor,
+                            ids: torch.Tensor) -> torch.Tensor:
+    return _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids)
+
+
+@_int8_adapter_linear_op.register_fake
+def _(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids):
+    return x.new_empty(*x.shape[:-1], weight.shape[0], dtype=torch.float16)
+
+
+def int8_adapter_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None,
+                        residual: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """adapter_linear beside the int8 linear (the op fry::int8_adapter_linear): x int8 [..., K] with x_scale fp32 a row,
+    weight int8 [N, K] with weight_scale fp32 a row, as int8_linear takes them; the adapters fp16, on the rows that x and
+    x_scale stand for. K a multiple of 16."""
+    run = _int8_adapter_linear if _direct(x, x_scale, weight_scale, bias, residual, down, up) else torch.ops.fry.int8_adapter_linear
+    return run(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids)
+
+
 @torch.library.custom_op("fry::norm_quant", mutates_args=())
 def norm_quant(x: torch.Tensor, gain: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """`chess::norm_quant` (model/int8_blocks.py:191-193): int8 rows of RMSNorm(x) * gain and their scales."""

@@ -74,6 +74,30 @@ int fry_int8_linear(const int8_t* x, const float* x_scale, const int8_t* weight,
 int fry_int8_linear_normed(const uint16_t* x, const uint16_t* gain, float eps, const int8_t* weight, const float* weight_scale,
                            const uint16_t* bias, uint16_t* out, int M, int N, int K, int gated, void* stream);
 
+/* fry_int8_linear with low-rank adapters of many requests: request s has the rows [offsets[s], offsets[s + 1]) and adapter
+ * a = ids[s] (offsets int32 [requests + 1] ascending, ids int32 [requests], both on the device; -1: none, as for rows of no
+ * request), and
+ *   out[m] = fp16((fma(acc * x_scale, weight_scale, bias) + (x_scale x[m] down[a]^T) up[a]^T) + residual[m])
+ * down fp16 [adapters, rank, K], up fp16 [adapters, N, rank] (a scale of the adapter is the caller's, in either); the
+ * adapters' sums fp32, x down^T rounded to fp16 between the two products. bias and residual fp16, either NULL: none. An
+ * adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids out of range are recorded in the device
+ * status (code 7, where = the request): ids count as -1, rows of such offsets hold unspecified values. rank a multiple of 8
+ * up to 128, N of 8, K of 16, adapters * N below 2^31, M and requests up to 2^24; out overlaps no input but residual;
+ * x, weight, down, up, residual, out and workspace 16-byte aligned. workspace: of fry_int8_adapter_linear_workspace_bytes;
+ * calls whose work overlaps on the GPU need workspaces of their own. No reference counterpart. */
+size_t fry_int8_adapter_linear_workspace_bytes(int M, int N, int requests, int rank);
+int fry_int8_adapter_linear(const int8_t* x, const float* x_scale, const int8_t* weight, const float* weight_scale, const uint16_t* bias,
+                            const uint16_t* residual, const uint16_t* down, const uint16_t* up, const int32_t* offsets, const int32_t* ids,
+                            uint16_t* out, int M, int N, int K, int requests, int adapters, int rank, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* The same beside fry_linear: x fp16 [M, K], weight fp16 [N, K], out[m] = fp16(((acc + (x[m] down[a]^T) up[a]^T) + bias) +
+ * residual[m]), the adapters in the linear's own fp32 sums. K a multiple of 8. */
+size_t fry_adapter_linear_workspace_bytes(int M, int N, int requests, int rank);
+int fry_adapter_linear(const uint16_t* x, const uint16_t* weight, const uint16_t* bias, const uint16_t* residual, const uint16_t* down,
+                       const uint16_t* up, const int32_t* offsets, const int32_t* ids, uint16_t* out, int M, int N, int K, int requests,
+                       int adapters, int rank, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The int32 sums x[M, K] . weight[N, K]^T of the same tensor-core kernel, for bit-exact checks. No reference
  * counterpart exposes them; they are the `acc` of model/int8_blocks.py:85-92. */
 int fry_int8_matmul_i32(const int8_t* x, const int8_t* weight, int32_t* out, int M, int N, int K, void* stream);

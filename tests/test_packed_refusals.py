@@ -92,3 +92,35 @@ def test_descending_starts_end_the_search_in_range():
     for _ in range(300):
         starts = [0] + [rng.randrange(500) for _ in range(rng.choice([1, 5, 40, 1100]))] + [500]
         assert all(0 <= find_segment(starts, 16, slot) <= len(starts) - 2 for slot in range(0, 500, 7))
+
+
+def adapters(lib, int8, M=4, N=16, K=32, requests=1, adapters=1, rank=8, x=16, scale=16, offsets=16, workspace=16, size=1 << 20):
+    pointer = ctypes.c_void_p
+    if int8:
+        return lib.fry_int8_adapter_linear(pointer(x), pointer(scale), pointer(16), pointer(scale), None, None, pointer(16), pointer(16), pointer(offsets),
+                                           pointer(16), pointer(16), M, N, K, requests, adapters, rank, pointer(workspace), size, None)
+    return lib.fry_adapter_linear(pointer(x), pointer(16), None, None, pointer(16), pointer(16), pointer(offsets), pointer(16), pointer(16), M, N, K,
+                                  requests, adapters, rank, pointer(workspace), size, None)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("arguments, match", [
+    ({"N": 12}, "multiple of 8"), ({"N": 0}, "multiple of 8"), ({"K": 20}, "K of"), ({"rank": 4}, "rank"), ({"rank": 136}, "rank"), ({"rank": 0}, "rank"),
+    ({"adapters": 0}, "1 or more"), ({"adapters": 1 << 28}, "2\\^31"), ({"M": -1}, "rows"), ({"requests": -1}, "requests"), ({"x": 8}, "16-byte"),
+    ({"x": None}, "needs x"), ({"offsets": None}, "offsets"), ({"workspace": None}, "workspace"), ({"size": 100}, "workspace"),
+])
+def test_linears_with_adapters_refuse(lib, int8, arguments, match):
+    with pytest.raises(FryError, match=match):
+        adapters(lib, int8, **arguments)
+
+
+def test_the_int8_linear_with_adapters_needs_its_scales(lib):
+    with pytest.raises(FryError, match="both scales"):
+        adapters(lib, True, scale=None)
+
+
+def test_linears_with_adapters_take_no_rows(lib):
+    assert adapters(lib, False, M=0) == adapters(lib, True, M=0) == 0
+    x = torch.zeros(3, 64, dtype=torch.float16)
+    with pytest.raises(FryError, match="GPU only"):
+        ops.adapter_linear(x, x, None, None, x[None], x[None], torch.tensor([0, 3], dtype=torch.int32), torch.tensor([0], dtype=torch.int32))
