@@ -77,7 +77,8 @@ int run_attention(const char* name, const fry::AttentionShape& shape, const fry:
     const size_t needed = fry::attention_plan(shape).workspace_bytes;
     if (needed > 0 && (!workspace || workspace_bytes < needed))
         return fail(FRY_ERROR_SHAPE, std::string(name) + "'s workspace is smaller than " + name + "_workspace_bytes");
-    return check(fry::packed_attention(shape, x, scale, workspace, as_stream(stream)), name);
+    std::string detail;
+    return check(fry::packed_attention(shape, x, scale, workspace, as_stream(stream), &detail), name, detail);
 }
 
 // Why the adapters' kernels do not take a shape ("" if they do).

@@ -138,13 +138,15 @@ struct AttentionTensors {
 // What the host chooses from the shape alone: the form, into how many blocks a row's keys are split, and the workspace
 // (the splits' partial results; 0 without a split).
 constexpr int kMaxAttentionSplits = 64;
+enum class AttentionForm { kFew, kRows, kPrompt };
 struct AttentionPlan {
-    bool few = false;
+    AttentionForm form = AttentionForm::kRows;
     int splits = 1;
     size_t workspace_bytes = 0;
 };
 AttentionPlan attention_plan(const AttentionShape& shape);
-cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& tensors, float scale, void* workspace, cudaStream_t stream);
+cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& tensors, float scale, void* workspace, cudaStream_t stream,
+                             std::string* error);
 
 // Heads (heads.cu).
 struct HeadWeights {

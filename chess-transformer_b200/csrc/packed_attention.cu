@@ -1,169 +1,14 @@
-// Attention over packed sequences and over a cache, on warp-wide tensor steps (mma.sync): out = softmax(scale q k^T) v for
-// each token and head, grouped heads (query head h reads key/value head h / group), causal or not.
-//
-//  packed: q [rows, heads, width], k and v [key rows, kv_heads, width], sequences one behind the other at q_offsets and
-//          k_offsets. Causal: a sequence's queries are its last tokens, query i sees keys j <= i + nk - nq.
-//  cached: q [sequences, heads, width], one token a sequence, k and v [sequences, capacity, kv_heads, width] of which the
-//          first lengths[s] keys count.
-//
-// Softmax in one pass over the keys: with m the running maximum of a row's scores (times scale log2 e) and l the running
-// sum of 2^(s - m), a tile of keys takes m to m' = max(m, its maximum), scales l and the row's sums o by 2^(m - m') and
-// adds its own 2^(s - m') and 2^(s - m') v. out = o / l at the end; a row that sees no key has l = 0 and answers 0. Scores,
-// m, l and o are fp32. The probabilities 2^(s - m') are rounded to the inputs' type for the second product (off by at most
-// half a step each, about what rounding the output costs), l sums them unrounded.
-//
-// Rows. The `group` query heads of a key/value head share its keys, so they are rows of one tile: row r of a block is token
-// r / group, head r % group, and one pass over the keys serves them all.
+// Attention over packed sequences and over a cache (packed_attention.cuh) on warp-wide tensor steps (mma.sync), for
+// sequences of few rows or few keys, and the choice between these kernels and those of prompt_attention.cu.
 //
 // Two forms. ROW_WARPS warps of 16 rows each share tiles of keys (many queries), or KEY_WARPS warps hold the same 16 rows
 // and take different keys, each with copies and a softmax of its own, joined at the end (few queries: there the loads
 // bound the kernel, and warps that wait for no other keep them in flight). Where blocks are still fewer than the SMs, the
 // keys are also split over blocks (`splits`): each writes its m, l and o to a workspace and attention_join_kernel joins
 // them in order of the split, so results do not depend on the blocks' order.
-//
-// What a query does not see does not reach it, whatever it holds: scores behind a row's last key count as -inf however
-// they came out, and rows behind a sequence's last key are read as zeros. A value of a key that some rows of a tile see
-// and others do not is multiplied by their probability 0; if it is not finite that product is NaN, so a row whose sum l is
-// finite and whose output is not is computed again over its own keys alone (recompute_row).
-#include <climits>
-
-#include "common.cuh"
-#include "kernels.h"
-#include "segments.cuh"
+#include "packed_attention.cuh"
 
 namespace fry {
-
-struct AttentionArgs {
-    const uint16_t *q, *k, *v;
-    uint16_t* out;                                         // [rows, heads, width] dense
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
-    int64_t k_sequence, v_sequence;                        // cached
-    int heads, kv_heads, width;
-    int group, tile_heads, head_tiles;  // query heads a key/value head, of which a block takes tile_heads in each of head_tiles
-    PackedRows queries;                 // packed; cached: count sequences of one row
-    const int32_t* k_offsets;           // packed: [count + 1]
-    int k_rows;
-    const int32_t* lengths;             // cached: [count], else null
-    int capacity;
-    int causal;
-    float scale_log2;                   // scale * log2(e), positive
-    int splits;
-    float* part_out;                    // [splits][rows][heads][width], where splits > 1
-    float* part_sums;                   // [splits][rows][heads][2]: m, l
-};
-
-// A block's rows: tokens [first, first + tokens) of a sequence of nq queries and nk keys.
-struct RowBlock {
-    int row;     // the first token's row of q and out
-    int first, tokens, nq, nk;
-    int64_t k_base, v_base;  // the sequence's first key and value, in elements
-    FRY_DEVICE int limit(int token, int causal) const {  // how many keys a token sees
-        if (!causal) return nk;
-        const int seen = nk - nq + first + token + 1;
-        return seen < 0 ? 0 : seen > nk ? nk : seen;
-    }
-};
-
-// The rows of block `slot` of tiles of `tile` tokens; false if it has none. Every thread of the warp calls it.
-FRY_DEVICE bool find_rows(const AttentionArgs& a, int tile, int slot, int lane, RowBlock& b) {
-    b.k_base = b.v_base = 0;
-    if (a.lengths) {
-        if (slot >= a.queries.count) return false;
-        const int length = a.lengths[slot];
-        b.row = slot, b.first = 0, b.tokens = 1, b.nq = 1;
-        b.nk = length < 0 ? 0 : length > a.capacity ? a.capacity : length;
-        if (b.nk != length && threadIdx.x == 0) record_error(kBadOffsets, slot);
-        b.k_base = slot * a.k_sequence, b.v_base = slot * a.v_sequence;
-        return true;
-    }
-    const int segment = find_segment(a.queries, tile, slot, lane);
-    const int start = a.queries.start(segment), end = a.queries.start(segment + 1);
-    b.first = (slot - start / tile - segment) * tile;
-    b.nq = end > start ? end - start : 0;
-    b.tokens = min(tile, b.nq - b.first);
-    if (b.tokens <= 0) return false;
-    b.row = start + b.first;
-    b.nk = 0;
-    if (segment >= 1 && segment <= a.queries.count) {  // not the rows before the first or behind the last sequence
-        const PackedRows keys{a.k_offsets, a.queries.count, a.k_rows};
-        const int k_start = keys.start(segment), k_end = keys.start(segment + 1);
-        b.nk = k_end > k_start ? k_end - k_start : 0;
-        b.k_base = k_start * a.k_row, b.v_base = k_start * a.v_row;
-    }
-    return true;
-}
-
-// Records a sequence whose offsets descend or leave their tensor. One block of a launch does it for all, the first: it has
-// the rows behind the last sequence, usually none.
-FRY_DEVICE void check_offsets(const AttentionArgs& a) {
-    if (a.lengths || blockIdx.x != 0 || blockIdx.y != 0 || blockIdx.z != 0) return;
-    const PackedRows keys{a.k_offsets, a.queries.count, a.k_rows};
-    for (int s = threadIdx.x; s < a.queries.count; s += blockDim.x)
-        if (a.queries.bad(s + 1) || keys.bad(s + 1)) record_error(kBadOffsets, s);
-}
-
-template <bool BF16>
-FRY_DEVICE float widen16(uint16_t bits) {
-    if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(bits) << 16);
-    else return h2f_bits(bits);
-}
-template <bool BF16>
-FRY_DEVICE uint32_t pack16(float lo, float hi) {
-    if constexpr (BF16) return pack_bf162_rn(lo, hi);
-    else return pack_half2_rn(lo, hi);
-}
-template <bool BF16>
-FRY_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16) mma_bf16(c, a, b0, b1);
-    else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
-}
-
-// Where a row's results go: out (o / l rounded), or with splits this split's m, l and o.
-struct AttentionOut {
-    uint16_t* out;
-    float *part_out, *part_sums;
-};
-FRY_DEVICE AttentionOut attention_out(const AttentionArgs& a, int split, int row, int head) {
-    const int64_t at = static_cast<int64_t>(row) * a.heads + head;
-    const int64_t part = static_cast<int64_t>(split) * a.queries.rows * a.heads + at;
-    return {a.out + at * a.width, a.part_out + part * a.width, a.part_sums + part * 2};
-}
-
-// One row by its definition, by a warp: softmax over keys [low, high) in tiles of 32, lane i summing columns i, i + 32, ...
-// Slow, for rows whose tile holds values that are not finite.
-template <bool BF16>
-__device__ __noinline__ void recompute_row(const AttentionArgs& a, const RowBlock& b, int token, int head, int low, int high, int split, int lane) {
-    const uint16_t* q = a.q + (b.row + token) * a.q_row + head * a.q_head;
-    const uint16_t* k = a.k + b.k_base + (head / a.group) * a.k_head;
-    const uint16_t* v = a.v + b.v_base + (head / a.group) * a.v_head;
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = low; j0 < high; j0 += 32) {
-        float s = -INFINITY;
-        if (j0 + lane < high) {
-            s = 0.0f;
-            for (int c = 0; c < a.width; ++c) s = __fmaf_rn(widen16<BF16>(q[c]), widen16<BF16>(k[(j0 + lane) * a.k_row + c]), s);
-            s *= a.scale_log2;
-        }
-        const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.0f : top;
-        const float p = j0 + lane < high ? ex2_approx(s - base) : 0.0f, shrink = ex2_approx(m - base);
-        l = l * shrink + warp_sum(p);
-        m = top;
-        for (int i = 0; i < 4; ++i) o[i] *= shrink;
-        for (int j = 0; j < 32 && j0 + j < high; ++j) {
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < a.width) o[i] = __fmaf_rn(pj, widen16<BF16>(v[(j0 + j) * a.v_row + lane + 32 * i]), o[i]);
-        }
-    }
-    const AttentionOut to = attention_out(a, split, b.row + token, head);
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane + 32 * i;
-        if (c >= a.width) continue;
-        if (a.splits > 1) to.part_out[c] = o[i];
-        else to.out[c] = static_cast<uint16_t>(pack16<BF16>(l == 0.0f ? 0.0f : o[i] / l, 0.0f) & 0xffff);
-    }
-    if (a.splits > 1 && lane == 0) to.part_sums[0] = m, to.part_sums[1] = l;
-}
 
 // Byte offset of 16-byte unit `unit` of row `row` in a tile of rows of WIDTH 16-bit values, so that eight rows' equal
 // units lie in different banks: rows of 128 bytes and up swap units by the row within 8, rows of 64 bytes are paired.
@@ -468,10 +313,13 @@ cudaError_t launch_width(const AttentionArgs& a, bool few, cudaStream_t stream) 
 }
 
 template <bool BF16>
-cudaError_t launch_type(const AttentionArgs& a, bool few, cudaStream_t stream) {
-    const cudaError_t status = a.width <= 32   ? launch_width<32, BF16>(a, few, stream)
-                               : a.width <= 64 ? launch_width<64, BF16>(a, few, stream)
-                                               : launch_width<128, BF16>(a, few, stream);
+cudaError_t launch_type(const AttentionArgs& a, AttentionForm form, cudaStream_t stream, std::string* error) {
+    const bool few = form == AttentionForm::kFew;
+    cudaError_t status;
+    if (form == AttentionForm::kPrompt) status = a.width <= 64 ? launch_prompt<64, BF16>(a, stream, error) : launch_prompt<128, BF16>(a, stream, error);
+    else if (a.width <= 32) status = launch_width<32, BF16>(a, few, stream);
+    else if (a.width <= 64) status = launch_width<64, BF16>(a, few, stream);
+    else status = launch_width<128, BF16>(a, few, stream);
     if (status != cudaSuccess || a.splits == 1) return status;
     const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads;
     return launch_dependent(attention_join_kernel<BF16>, dim3(static_cast<unsigned>((count + 3) / 4)), dim3(128), 0, stream, a);
@@ -483,11 +331,12 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     AttentionPlan plan;
     const int64_t sequences = s.sequences > 0 ? s.sequences : 1;
     const int64_t mean_rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / sequences, mean_keys = s.cached ? s.capacity : s.key_rows / sequences;
-    plan.few = s.cached || mean_rows <= 16;
+    const bool few = s.cached || mean_rows <= 16, prompt = !few && mean_rows >= 128 && mean_keys >= 128;
+    plan.form = few ? AttentionForm::kFew : prompt ? AttentionForm::kPrompt : AttentionForm::kRows;
     // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
-    const int64_t group = s.heads / s.kv_heads, rows = plan.few ? 16 : 64, tile = rows / (group < rows ? group : rows);
+    const int64_t group = s.heads / s.kv_heads, rows = few ? 16 : prompt ? 256 : 64, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
-    const int64_t wanted = 2 * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    const int64_t wanted = (prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
     const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;
@@ -495,7 +344,7 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     return plan;
 }
 
-cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& x, float scale, void* workspace, cudaStream_t stream) {
+cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& x, float scale, void* workspace, cudaStream_t stream, std::string* error) {
     const AttentionPlan plan = attention_plan(shape);
     AttentionArgs a = {};
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
@@ -510,7 +359,7 @@ cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors
     a.splits = plan.splits;
     a.part_sums = static_cast<float*>(workspace);
     a.part_out = a.part_sums + static_cast<size_t>(plan.splits) * shape.q_rows * shape.heads * 2;
-    return shape.bf16 ? launch_type<true>(a, plan.few, stream) : launch_type<false>(a, plan.few, stream);
+    return shape.bf16 ? launch_type<true>(a, plan.form, stream, error) : launch_type<false>(a, plan.form, stream, error);
 }
 
 }  // namespace fry
