@@ -130,7 +130,7 @@ FRY_DEVICE AttentionOut attention_out(const AttentionArgs& a, int split, int row
 // One row by its definition, by a warp: softmax over keys [low, high) in tiles of 32, lane i summing columns i, i + 32, ...
 // Slow, for rows whose tile holds values that are not finite.
 template <bool BF16>
-__device__ __noinline__ void recompute_row(const AttentionArgs& a, const RowBlock& b, int token, int head, int low, int high, int split, int lane) {
+FRY_DEVICE void recompute_row(const AttentionArgs& a, const RowBlock& b, int token, int head, int low, int high, int split, int lane) {
     const uint16_t* q = a.q + (b.row + token) * a.q_row + head * a.q_head;
     const uint16_t* k = a.k + b.k_base + (head / a.group) * a.k_head;
     const uint16_t* v = a.v + b.v_base + (head / a.group) * a.v_head;

@@ -23,7 +23,10 @@
 namespace fry {
 
 constexpr int kPromptTile = 128;                // rows of a tile, and keys of a stage
-constexpr int kPromptSoftmaxWarps = 8, kPromptLoadWarp = 8, kPromptMmaWarp = 9, kPromptThreads = 10 * 32;
+constexpr int kPromptSoftmaxWarps = 8, kPromptLoadWarp = 8, kPromptMmaWarp = 9, kPromptThreads = 12 * 32;
+// Registers a thread: the launch gives 168 to each of the three groups of four warps (384 threads x 168 = 64512); the
+// softmax's two groups take 208, which hold a row's 128 scores, the third keeps 88 (2 x 128 x 208 + 128 x 88 = 64512).
+constexpr int kPromptSoftmaxRegisters = 208, kPromptOtherRegisters = 88;
 constexpr float kLagLog2 = 8.0f;
 
 template <int WIDTH>
@@ -101,15 +104,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     uint64_t* full = q_full + 1;                          // [kStages]
     uint64_t* empty = full + S::kStages;                  // [kStages]
     uint64_t* s_full = empty + S::kStages;                // [2]: a tile's scores are there, and its last P V is done
-    uint64_t* p_full = s_full + 2;                        // [2]: its probabilities are
-    uint64_t* o_full = p_full + 2;                        // [2]: its output is
+    uint64_t* p_full = s_full + 2;                        // [2][2]: the first and second half of its probabilities are
+    uint64_t* o_full = p_full + 4;                        // [2]: its output is
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < S::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&p_full[t], kPromptSoftmaxWarps / 2), mbar_init(&o_full[t], 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&o_full[t], 1);
+        for (int h = 0; h < 4; ++h) mbar_init(&p_full[h], kPromptSoftmaxWarps / 2);
         fence_barrier_init();
     }
     grid_dependency_start();
@@ -156,69 +160,76 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == kPromptLoadWarp) {
-        if (elect_one()) {
-            const int tiles = counts[1] > 0 ? 2 : 1;
-            // a box has whole tokens: tile * tile_heads rows of the 128
-            mbar_arrive_expect_tx(q_full, tiles * (WIDTH / 64) * tile * a.tile_heads * 128);
-            for (int t = 0; t < tiles; ++t)
-                for (int box = 0; box < WIDTH / 64; ++box)
-                    tma_load_4d(queries + t * S::kTileBytes + box * S::kBoxBytes, &map_q, q_full, box * 64, head_tile * a.tile_heads, b.row + t * tile, kv_head);
-            bool ok = true;
-            for (int i = 0; i < 2 * steps && ok; ++i) {  // keys and values of a step in turn
-                const int s = i % S::kStages;
-                ok = mbar_wait(&empty[s], ((i / S::kStages) & 1) ^ 1, 31);
-                if (!ok) break;
-                mbar_arrive_expect_tx(&full[s], S::kTileBytes);
-                for (int box = 0; box < WIDTH / 64; ++box)
-                    tma_load_3d(stages + s * S::kTileBytes + box * S::kBoxBytes, i & 1 ? &map_v : &map_k, &full[s], box * 64,
-                                b.k_first + low + (i >> 1) * kPromptTile, kv_head);
-            }
-        }
-    } else if (warp == kPromptMmaWarp) {
-        if (elect_one()) {
-            constexpr uint32_t score_desc = prompt_desc<BF16>(kPromptTile, false), out_desc = prompt_desc<BF16>(WIDTH, true);
-            auto stage = [&](int i) { return smem_addr(stages + (i % S::kStages) * S::kTileBytes); };
-            auto wait_stage = [&](int i) { return mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, 32); };
-            auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
-                const uint32_t q = smem_addr(queries + t * S::kTileBytes), k = stage(2 * j);
-#pragma unroll
-                for (int c = 0; c < WIDTH / 16; ++c) {
-                    const uint32_t offset = (c / 4) * S::kBoxBytes + (c % 4) * 32;
-                    mma_ss<1>(tmem + t * kPromptTile, smem_desc_sw128(q + offset), smem_desc_sw128(k + offset), score_desc, c > 0 ? 1u : 0u);
-                }
-                mma_commit(&s_full[t]);
-            };
-            bool ok = mbar_wait(q_full, 0, 33) && wait_stage(0);
-            tc_fence_after();
-            if (ok) {
-                for (int t = 0; t < 2; ++t)
-                    if (counts[t] > 0) scores(t, 0);
-                mma_commit(&empty[0]);
-            }
-            for (int j = 0; j < steps && ok; ++j) {
-                const int v_stage = 2 * j + 1, k_next = 2 * j + 2;
-                ok = wait_stage(v_stage) && (j + 1 >= steps || wait_stage(k_next));
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (j >= counts[t]) continue;
-                    ok = mbar_wait(&p_full[t], j & 1, 34);
+    if (warp >= kPromptSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegisters));
+        if (warp == kPromptLoadWarp) {
+            if (elect_one()) {
+                const int tiles = counts[1] > 0 ? 2 : 1;
+                // a box has whole tokens: tile * tile_heads rows of the 128
+                mbar_arrive_expect_tx(q_full, tiles * (WIDTH / 64) * tile * a.tile_heads * 128);
+                for (int t = 0; t < tiles; ++t)
+                    for (int box = 0; box < WIDTH / 64; ++box)
+                        tma_load_4d(queries + t * S::kTileBytes + box * S::kBoxBytes, &map_q, q_full, box * 64, head_tile * a.tile_heads, b.row + t * tile, kv_head);
+                bool ok = true;
+                for (int i = 0; i < 2 * steps && ok; ++i) {  // keys and values of a step in turn
+                    const int s = i % S::kStages;
+                    ok = mbar_wait(&empty[s], ((i / S::kStages) & 1) ^ 1, 31);
                     if (!ok) break;
-                    tc_fence_after();
-                    // O_t += P_t V_j over the keys the tile sees, 16 an MMA
-                    const int keys = min(kPromptTile, highs[t] - low - j * kPromptTile), chunks = (keys + 15) / 16;
-                    for (int c = 0; c < chunks; ++c)
-                        mma_ts(tmem + 2 * kPromptTile + t * WIDTH, tmem + t * kPromptTile + c * 8, value_desc(stage(v_stage) + c * 16 * 128), out_desc,
-                               j > 0 || c > 0 ? 1u : 0u);
-                    if (j + 1 < counts[t]) scores(t, j + 1);
-                    else mma_commit(&o_full[t]);
+                    mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+                    for (int box = 0; box < WIDTH / 64; ++box)
+                        tma_load_3d(stages + s * S::kTileBytes + box * S::kBoxBytes, i & 1 ? &map_v : &map_k, &full[s], box * 64,
+                                    b.k_first + low + (i >> 1) * kPromptTile, kv_head);
                 }
+            }
+        } else if (warp == kPromptMmaWarp) {
+            if (elect_one()) {
+                constexpr uint32_t score_desc = prompt_desc<BF16>(kPromptTile, false), out_desc = prompt_desc<BF16>(WIDTH, true);
+                auto stage = [&](int i) { return smem_addr(stages + (i % S::kStages) * S::kTileBytes); };
+                auto wait_stage = [&](int i) { return mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, 32); };
+                auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
+                    const uint32_t q = smem_addr(queries + t * S::kTileBytes), k = stage(2 * j);
+#pragma unroll
+                    for (int c = 0; c < WIDTH / 16; ++c) {
+                        const uint32_t offset = (c / 4) * S::kBoxBytes + (c % 4) * 32;
+                        mma_ss<1>(tmem + t * kPromptTile, smem_desc_sw128(q + offset), smem_desc_sw128(k + offset), score_desc, c > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&s_full[t]);
+                };
+                bool ok = mbar_wait(q_full, 0, 33) && wait_stage(0);
+                tc_fence_after();
                 if (ok) {
-                    mma_commit(&empty[v_stage % S::kStages]);
-                    if (j + 1 < steps) mma_commit(&empty[k_next % S::kStages]);
+                    for (int t = 0; t < 2; ++t)
+                        if (counts[t] > 0) scores(t, 0);
+                    mma_commit(&empty[0]);
+                }
+                for (int j = 0; j < steps && ok; ++j) {
+                    const int v_stage = 2 * j + 1, k_next = 2 * j + 2;
+                    ok = wait_stage(v_stage) && (j + 1 >= steps || wait_stage(k_next));
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j >= counts[t]) continue;
+                        // O_t += P_t V_j over the keys the tile sees, 16 an MMA, in the halves that P comes in
+                        const int keys = min(kPromptTile, highs[t] - low - j * kPromptTile), chunks = (keys + 15) / 16;
+                        for (int half = 0; half < 2 && ok; ++half) {
+                            ok = mbar_wait(&p_full[2 * t + half], j & 1, 34);
+                            if (!ok) break;
+                            tc_fence_after();
+                            for (int c = 4 * half; c < min(chunks, 4 * half + 4); ++c)
+                                mma_ts(tmem + 2 * kPromptTile + t * WIDTH, tmem + t * kPromptTile + c * 8, value_desc(stage(v_stage) + c * 16 * 128), out_desc,
+                                       j > 0 || c > 0 ? 1u : 0u);
+                        }
+                        if (!ok) break;
+                        if (j + 1 < counts[t]) scores(t, j + 1);
+                        else mma_commit(&o_full[t]);
+                    }
+                    if (ok) {
+                        mma_commit(&empty[v_stage % S::kStages]);
+                        if (j + 1 < steps) mma_commit(&empty[k_next % S::kStages]);
+                    }
                 }
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegisters));
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // this thread's row of tile t
         const int count = counts[t];
         const int token = t * tile + row / a.tile_heads, in_group = head_tile * a.tile_heads + row % a.tile_heads;
@@ -229,7 +240,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const uint32_t lanes_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + t * kPromptTile + lanes_at, o_tmem = tmem + 2 * kPromptTile + t * WIDTH + lanes_at;
         float m = -INFINITY;
-        uint64_t total2 = pair2(0.0f, 0.0f);
+        uint64_t totals[2] = {pair2(0.0f, 0.0f), pair2(0.0f, 0.0f)};
         bool alive = true;
         for (int j = 0; j < count; ++j) {
             if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, 35))) {
@@ -262,7 +273,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const float shrink = ex2_approx_ftz(m - (risen == -INFINITY ? 0.0f : risen));
                 const uint64_t shrink2 = pair2(shrink, shrink);
                 m = risen;
-                total2 = mul2(total2, shrink2);
+                totals[0] = mul2(totals[0], shrink2), totals[1] = mul2(totals[1], shrink2);
                 if (j > 0) {  // O is complete up to the keys before these
 #pragma unroll 1
                     for (int c = 0; c < WIDTH; c += 32) {
@@ -275,21 +286,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : -m;
-            const uint64_t base2 = pair2(base, base), scale2 = pair2(a.scale_log2, a.scale_log2);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t packed[32];
-#pragma unroll
-                for (int e = 0; e < 64; e += 2) {
-                    const uint32_t* from = &raw[half * 2 + e / 32][e % 32];
-                    const float2 x = lanes(fma2(pair2(__uint_as_float(from[0]), __uint_as_float(from[1])), scale2, base2));
-                    const float2 p = make_float2(ex2_approx_ftz(x.x), ex2_approx_ftz(x.y));
-                    total2 = add2(total2, pair2(p.x, p.y));
-                    packed[e / 2] = pack16<BF16>(p.x, p.y);
-                }
-                tmem_store32(s_tmem + half * 32, packed);
-            }
             // value rows behind the sequence's last key that the last MMA's 16 keys still take are another sequence's: zeros
             if (first_key + kPromptTile > b.nk && (highs[t] - first_key + 15) / 16 * 16 > b.nk - first_key) {
                 const int i = 2 * j + 1;
@@ -300,14 +296,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     *reinterpret_cast<uint4*>(values + (u % (WIDTH / 8)) / 8 * S::kBoxBytes + (from + u / (WIDTH / 8)) * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_shared();
             }
-            tmem_store_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            const float base = m == -INFINITY ? 0.0f : -m;
+            const uint64_t base2 = pair2(base, base), scale2 = pair2(a.scale_log2, a.scale_log2);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    const uint32_t* from = &raw[half * 2 + e / 32][e % 32];
+                    const float2 x = lanes(fma2(pair2(__uint_as_float(from[0]), __uint_as_float(from[1])), scale2, base2));
+                    const float2 p = make_float2(ex2_approx_ftz(x.x), ex2_approx_ftz(x.y));
+                    totals[e / 2 % 2] = add2(totals[e / 2 % 2], pair2(p.x, p.y));
+                    packed[e / 2] = pack16<BF16>(p.x, p.y);
+                }
+                tmem_store32(s_tmem + half * 32, packed);
+                tmem_store_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
+            }
         }
         if (count > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, 37));
         tc_fence_after();
-        const float2 both = lanes(total2);
+        const float2 both = lanes(add2(totals[0], totals[1]));
         const float total = both.x + both.y, inverse = total == 0.0f ? 0.0f : 1.0f / total;
         const int head = kv_head * a.group + in_group;
         const AttentionOut to = attention_out(a, split, b.row + token, head);
