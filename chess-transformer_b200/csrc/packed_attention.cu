@@ -33,8 +33,11 @@ struct RowsShape {
     static constexpr int kTileBytes = kStageKeys * WIDTH * 2;  // the keys or the values of a stage
     static constexpr int kLoopBytes = STAGES * 2 * kTileBytes;
     // after the loop: a warp's 16 output rows, or with KEY_WARPS its 16 rows of fp32 sums, m and l
-    static constexpr int kJoinBytes = KEY_WARPS > 1 ? KEY_WARPS * 16 * (WIDTH + 2) * 4 : ROW_WARPS * 16 * WIDTH * 2;
-    static constexpr int kSmemBytes = kLoopBytes > kJoinBytes ? kLoopBytes : kJoinBytes;
+    static constexpr int kSumsPitch = WIDTH + 8;  // floats a row: the quads of a store in different banks
+    static constexpr int kJoinBytes = KEY_WARPS > 1 ? KEY_WARPS * 16 * (kSumsPitch + 2) * 4 : ROW_WARPS * 16 * WIDTH * 2;
+    static constexpr int kFoundAt = kLoopBytes > kJoinBytes ? kLoopBytes : kJoinBytes;  // the block's RowBlock
+    static constexpr int kSmemBytes = kFoundAt + 64;
+    static_assert(sizeof(RowBlock) <= 64, "the block's rows fit their place");
 };
 
 template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
@@ -47,15 +50,23 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
     check_offsets(a);
 
     const int tile = S::kRows / a.tile_heads;  // tokens a block
-    RowBlock b;
-    // later tokens see more keys: they start first
-    if (!find_rows(a, tile, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, b)) return;
+    // later tokens see more keys: they start first. One warp searches for all.
+    RowBlock* found = reinterpret_cast<RowBlock*>(smem + S::kFoundAt);
+    if (warp == 0) {
+        RowBlock mine;
+        if (!find_rows(a, tile, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, mine)) mine.tokens = 0;
+        if (lane == 0) *found = mine;
+    }
+    __syncthreads();
+    const RowBlock b = *found;
+    if (b.tokens <= 0) return;
     const int kv_head = blockIdx.y / a.head_tiles, first_head = kv_head * a.group + (blockIdx.y % a.head_tiles) * a.tile_heads;
     const int heads_here = min(a.tile_heads, (kv_head + 1) * a.group - first_head);
     // a row's token and head; rows past the block's tokens or heads compute on zeros and are not written
     auto token_of = [&](int r) { return r / a.tile_heads; };
     auto head_of = [&](int r) { return first_head + r % a.tile_heads; };
     auto live = [&](int r) { return r / a.tile_heads < b.tokens && r % a.tile_heads < heads_here; };
+    const bool idle = row_warp * 16 >= b.tokens * a.tile_heads;  // no row of this warp's 16 is live
 
     // this block's keys: those its last token sees, of which a split takes whole stages
     const int seen = b.limit(b.tokens - 1, a.causal);
@@ -113,10 +124,13 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         else __syncthreads();
         load(step + STAGES - 1);  // into the stage read in the step before, which every reader has left
         const uint32_t k_tile = smem_addr(smem + (step % STAGES) * 2 * S::kTileBytes), v_tile = k_tile + S::kTileBytes;
+        if (idle) continue;
+        const int first_key = low + step * S::kStageKeys + key_warp * KEYS, left = high - first_key;  // this warp's keys
         float s[KEYS / 8][4] = {};
         const int key_row = key_warp * KEYS + (lane >> 4) * 8 + (lane & 7), key_unit = (lane >> 3) & 1;
 #pragma unroll
-        for (int n = 0; n < KEYS / 16; ++n)
+        for (int n = 0; n < KEYS / 16; ++n) {
+            if (n * 16 >= left) break;  // 16 keys at a time, none behind the last
 #pragma unroll
             for (int c = 0; c < WIDTH / 16; ++c) {
                 uint32_t f[4];
@@ -124,8 +138,7 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
                 mma16816<BF16>(s[2 * n], q[c], f[0], f[1]);
                 mma16816<BF16>(s[2 * n + 1], q[c], f[2], f[3]);
             }
-        // keys from this one on are behind a row's last
-        const int first_key = low + step * S::kStageKeys + key_warp * KEYS;
+        }
         if (first_key + KEYS > min(min(limit[0], limit[1]), high)) {
 #pragma unroll
             for (int n = 0; n < KEYS / 8; ++n)
@@ -137,24 +150,32 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         for (int half = 0; half < 2; ++half) {
             float top = s[0][2 * half];
 #pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
+            for (int n = 0; n < KEYS / 8; ++n) {
+                if (n % 2 == 0 && n * 8 >= left) break;
+                top = max3(top, s[n][2 * half], s[n][2 * half + 1]);
+            }
             top = fmaxf(m[half], quad_max(top) * a.scale_log2);
             const float base = top == -INFINITY ? 0.0f : top, shrink = ex2_approx_ftz(m[half] - base);
             m[half] = top;
             l[half] *= shrink;
 #pragma unroll
             for (int c = 0; c < WIDTH / 8; ++c) o[c][2 * half] *= shrink, o[c][2 * half + 1] *= shrink;
+            const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), base2 = pair2(-base, -base);
+            uint64_t total2 = pair2(0.0f, 0.0f);
 #pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n)
-#pragma unroll
-                for (int e = 2 * half; e < 2 * half + 2; ++e) {
-                    s[n][e] = ex2_approx_ftz(__fmaf_rn(s[n][e], a.scale_log2, -base));
-                    l[half] += s[n][e];
-                }
+            for (int n = 0; n < KEYS / 8; ++n) {
+                if (n % 2 == 0 && n * 8 >= left) break;
+                const float2 x = lanes(fma2(pair2(s[n][2 * half], s[n][2 * half + 1]), scale2, base2));
+                s[n][2 * half] = ex2_approx_ftz(x.x), s[n][2 * half + 1] = ex2_approx_ftz(x.y);
+                total2 = add2(total2, pair2(s[n][2 * half], s[n][2 * half + 1]));
+            }
+            const float2 total = lanes(total2);
+            l[half] += total.x + total.y;
         }
         const int value_row = key_warp * KEYS + ((lane >> 3) & 1) * 8 + (lane & 7), value_unit = lane >> 4;
 #pragma unroll
         for (int n = 0; n < KEYS / 16; ++n) {
+            if (n * 16 >= left) break;
             const uint32_t p[4] = {pack16<BF16>(s[2 * n][0], s[2 * n][1]), pack16<BF16>(s[2 * n][2], s[2 * n][3]),
                                    pack16<BF16>(s[2 * n + 1][0], s[2 * n + 1][1]), pack16<BF16>(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
@@ -173,14 +194,14 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
 
     if constexpr (KEY_WARPS > 1) {
         float* sums = reinterpret_cast<float*>(smem);             // [KEY_WARPS][16][2]: m, l
-        float* tops = sums + KEY_WARPS * 16 * 2;                  // [KEY_WARPS][16][WIDTH]
+        float* tops = sums + KEY_WARPS * 16 * 2;                  // [KEY_WARPS][16][kSumsPitch]
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int r = g + 8 * half;
             if (t == 0) sums[(warp * 16 + r) * 2] = m[half], sums[(warp * 16 + r) * 2 + 1] = l[half];
 #pragma unroll
             for (int c = 0; c < WIDTH / 8; ++c)
-                *reinterpret_cast<float2*>(tops + (warp * 16 + r) * WIDTH + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
+                *reinterpret_cast<float2*>(tops + (warp * 16 + r) * S::kSumsPitch + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
         }
         __syncthreads();
         for (int r = warp; r < 16; r += KEY_WARPS) {  // a warp a row, lane i columns i, i + 32, ...
@@ -194,7 +215,7 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
                 const float share = ex2_approx_ftz(sums[(w * 16 + r) * 2] - base);
                 total = __fmaf_rn(share, sums[(w * 16 + r) * 2 + 1], total);
 #pragma unroll
-                for (int i = 0; i < WIDTH / 32; ++i) joined[i] = __fmaf_rn(share, tops[(w * 16 + r) * WIDTH + lane + 32 * i], joined[i]);
+                for (int i = 0; i < WIDTH / 32; ++i) joined[i] = __fmaf_rn(share, tops[(w * 16 + r) * S::kSumsPitch + lane + 32 * i], joined[i]);
             }
             bool finite = true;
 #pragma unroll
@@ -262,33 +283,46 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
     }
 }
 
-// Joins the splits of each (row, head), a warp each, in the order of the splits: with M the largest m,
-// out = sum 2^(m - M) o / sum 2^(m - M) l.
+// Joins the splits of a (row, head), a block each: with M the largest m, out = sum 2^(m - M) o / sum 2^(m - M) l. Warp w
+// takes splits w, w + 4, ..., whose loads do not wait for one another; the warps' sums are added in order.
+constexpr int kJoinWarps = 4;
 template <bool BF16>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttentionArgs a) {
-    const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttentionArgs a) {
+    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float totals[kJoinWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependency_start();
-    const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads, at = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (at >= count) return;
-    float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_sums[(s * count + at) * 2]);
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 sums = *reinterpret_cast<const float2*>(a.part_sums + (s * count + at) * 2);
-        if (sums.y == 0.0f) continue;  // a split without keys for this row
-        const float share = ex2_approx_ftz(sums.x - base);
-        total = __fmaf_rn(share, sums.y, total);
-        const float* part = a.part_out + (s * count + at) * a.width;
+    const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads, at = blockIdx.x;
+    // lane i holds m and l of splits i and i + 32
+    static_assert(kMaxAttentionSplits <= 64, "two splits a lane");
+    float2 mine[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.width) o[i] = __fmaf_rn(share, part[lane + 32 * i], o[i]);
+    for (int i = 0; i < 2; ++i)
+        mine[i] = lane + 32 * i < a.splits ? *reinterpret_cast<const float2*>(a.part_sums + ((lane + 32 * i) * count + at) * 2) : make_float2(-INFINITY, 0.0f);
+    const float top = warp_max(fmaxf(mine[0].x, mine[1].x)), base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += kJoinWarps) {
+        const float m = __shfl_sync(0xffffffffu, s < 32 ? mine[0].x : mine[1].x, s & 31), l = __shfl_sync(0xffffffffu, s < 32 ? mine[0].y : mine[1].y, s & 31);
+        const float share = ex2_approx_ftz(m - base);
+        float4 part = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a split without keys for this row has written no output
+        if (l != 0.0f && 4 * lane < a.width) part = reinterpret_cast<const float4*>(a.part_out + (s * count + at) * a.width)[lane];
+        total = __fmaf_rn(share, l, total);
+        o.x = __fmaf_rn(share, part.x, o.x), o.y = __fmaf_rn(share, part.y, o.y), o.z = __fmaf_rn(share, part.z, o.z), o.w = __fmaf_rn(share, part.w, o.w);
+    }
+    sums[warp][lane] = o;
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    if (warp != 0 || 4 * lane >= a.width) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) {
+        const float4 other = sums[w][lane];
+        o.x += other.x, o.y += other.y, o.z += other.z, o.w += other.w;
+        total += totals[w];
     }
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.width) a.out[at * a.width + lane + 32 * i] = static_cast<uint16_t>(pack16<BF16>(o[i] * inverse, 0.0f) & 0xffff);
+    reinterpret_cast<uint2*>(a.out + at * a.width)[lane] = make_uint2(pack16<BF16>(o.x * inverse, o.y * inverse), pack16<BF16>(o.z * inverse, o.w * inverse));
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------
@@ -322,7 +356,7 @@ cudaError_t launch_type(const AttentionArgs& a, AttentionForm form, cudaStream_t
     else status = launch_width<128, BF16>(a, few, stream);
     if (status != cudaSuccess || a.splits == 1) return status;
     const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads;
-    return launch_dependent(attention_join_kernel<BF16>, dim3(static_cast<unsigned>((count + 3) / 4)), dim3(128), 0, stream, a);
+    return launch_dependent(attention_join_kernel<BF16>, dim3(static_cast<unsigned>(count)), dim3(kJoinWarps * 32), 0, stream, a);
 }
 
 }  // namespace
@@ -336,7 +370,7 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
     const int64_t group = s.heads / s.kv_heads, rows = few ? 16 : prompt ? 256 : 64, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
-    const int64_t wanted = (prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    const int64_t wanted = (s.cached ? 16 : prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
     const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;

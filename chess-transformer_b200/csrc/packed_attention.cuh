@@ -116,6 +116,12 @@ FRY_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uin
     else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
 }
 
+FRY_DEVICE float max3(float a, float b, float c) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
 // Where a row's results go: out (o / l rounded), or with splits this split's m, l and o.
 struct AttentionOut {
     uint16_t* out;

@@ -82,11 +82,6 @@ template <bool BF16>
 __host__ __device__ constexpr uint32_t prompt_desc(int n, bool rows_are_k) {
     return instr_desc<1>(n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (rows_are_k ? 1u << 16 : 0u);
 }
-FRY_DEVICE float max3(float a, float b, float c) {
-    float m;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
-    return m;
-}
 
 template <int WIDTH, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1)
