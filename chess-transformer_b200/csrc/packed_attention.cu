@@ -63,9 +63,9 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
     const int kv_head = blockIdx.y / a.head_tiles, first_head = kv_head * a.group + (blockIdx.y % a.head_tiles) * a.tile_heads;
     const int heads_here = min(a.tile_heads, (kv_head + 1) * a.group - first_head);
     // a row's token and head; rows past the block's tokens or heads compute on zeros and are not written
-    auto token_of = [&](int r) { return r / a.tile_heads; };
-    auto head_of = [&](int r) { return first_head + r % a.tile_heads; };
-    auto live = [&](int r) { return r / a.tile_heads < b.tokens && r % a.tile_heads < heads_here; };
+    auto token_of = [&](int r) { return a.token_of(r); };
+    auto head_of = [&](int r) { return first_head + a.head_in_tile(r); };
+    auto live = [&](int r) { return a.token_of(r) < b.tokens && a.head_in_tile(r) < heads_here; };
     const bool idle = row_warp * 16 >= b.tokens * a.tile_heads;  // no row of this warp's 16 is live
 
     // this block's keys: those its last token sees, of which a split takes whole stages
@@ -108,13 +108,23 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
     for (int half = 0; half < 2; ++half) {
         const int r = row_warp * 16 + g + 8 * half;
         const bool mine = live(r);
-        limit[half] = mine ? b.limit(token_of(r), a.causal) : INT_MAX;
+        limit[half] = mine ? min(high, b.limit(token_of(r), a.causal)) : high;
         const uint16_t* row = a.q + (mine ? (b.row + token_of(r)) * a.q_row + head_of(r) * a.q_head : 0);
 #pragma unroll
         for (int s = 0; s < WIDTH / 16; ++s)
 #pragma unroll
             for (int part = 0; part < 2; ++part)
                 q[s][half + 2 * part] = mine && 2 * s + part < units ? *reinterpret_cast<const uint32_t*>(row + s * 16 + part * 8 + 2 * t) : 0u;
+    }
+
+    // where this lane's rows of the B fragments lie: units swap within 8 (or 16) rows alike, so 16 keys on is a fixed step
+    const int key_row = key_warp * KEYS + (lane >> 4) * 8 + (lane & 7), value_row = key_warp * KEYS + ((lane >> 3) & 1) * 8 + (lane & 7);
+    const uint32_t k_offset = tile_unit<WIDTH>(key_row, 0) & ~127u, v_offset = tile_unit<WIDTH>(value_row, 0) & ~127u;
+    uint32_t k_units[WIDTH / 16], v_units[WIDTH / 16];
+#pragma unroll
+    for (int c = 0; c < WIDTH / 16; ++c) {
+        k_units[c] = tile_unit<WIDTH>(key_row, 2 * c + ((lane >> 3) & 1)) - k_offset;
+        v_units[c] = tile_unit<WIDTH>(value_row, 2 * c + (lane >> 4)) - v_offset;
     }
 
     float o[WIDTH / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -127,24 +137,27 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         if (idle) continue;
         const int first_key = low + step * S::kStageKeys + key_warp * KEYS, left = high - first_key;  // this warp's keys
         float s[KEYS / 8][4] = {};
-        const int key_row = key_warp * KEYS + (lane >> 4) * 8 + (lane & 7), key_unit = (lane >> 3) & 1;
+        const uint32_t k_lane = k_tile + k_offset, v_lane = v_tile + v_offset;
 #pragma unroll
         for (int n = 0; n < KEYS / 16; ++n) {
             if (n * 16 >= left) break;  // 16 keys at a time, none behind the last
 #pragma unroll
             for (int c = 0; c < WIDTH / 16; ++c) {
                 uint32_t f[4];
-                ldmatrix_x4(k_tile + tile_unit<WIDTH>(key_row + n * 16, 2 * c + key_unit), f);
+                ldmatrix_x4(k_lane + n * 16 * WIDTH * 2 + k_units[c], f);
                 mma16816<BF16>(s[2 * n], q[c], f[0], f[1]);
                 mma16816<BF16>(s[2 * n + 1], q[c], f[2], f[3]);
             }
         }
-        if (first_key + KEYS > min(min(limit[0], limit[1]), high)) {
+        if (first_key + KEYS > min(limit[0], limit[1])) {
+            const int seen_here[2] = {limit[0] - first_key - 2 * t, limit[1] - first_key - 2 * t};
 #pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n)
+            for (int n = 0; n < KEYS / 8; ++n) {
+                if (n % 2 == 0 && n * 8 >= left) break;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (first_key + n * 8 + 2 * t + (e & 1) >= min(limit[e >> 1], high)) s[n][e] = -INFINITY;
+                    if (n * 8 + (e & 1) >= seen_here[e >> 1]) s[n][e] = -INFINITY;
+            }
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -172,7 +185,6 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
             const float2 total = lanes(total2);
             l[half] += total.x + total.y;
         }
-        const int value_row = key_warp * KEYS + ((lane >> 3) & 1) * 8 + (lane & 7), value_unit = lane >> 4;
 #pragma unroll
         for (int n = 0; n < KEYS / 16; ++n) {
             if (n * 16 >= left) break;
@@ -181,7 +193,7 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
 #pragma unroll
             for (int c = 0; c < WIDTH / 16; ++c) {
                 uint32_t f[4];
-                ldmatrix_x4_trans(v_tile + tile_unit<WIDTH>(value_row + n * 16, 2 * c + value_unit), f);
+                ldmatrix_x4_trans(v_lane + n * 16 * WIDTH * 2 + v_units[c], f);
                 mma16816<BF16>(o[2 * c], p, f[0], f[1]);
                 mma16816<BF16>(o[2 * c + 1], p, f[2], f[3]);
             }
@@ -332,8 +344,7 @@ namespace {
 template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
 cudaError_t launch_rows(AttentionArgs a, cudaStream_t stream) {
     using S = RowsShape<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES>;
-    a.tile_heads = a.group < S::kRows ? a.group : S::kRows;
-    a.head_tiles = (a.group + a.tile_heads - 1) / a.tile_heads;
+    a.set_tile(S::kRows);
     const int slots = a.lengths ? a.queries.count : packed_slots(a.queries.rows, S::kRows / a.tile_heads, a.queries.count);
     auto kernel = attention_rows_kernel<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES, BF16>;
     const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);

@@ -37,6 +37,14 @@ struct AttentionArgs {
     int64_t k_sequence, v_sequence;                        // cached
     int heads, kv_heads, width;
     int group, tile_heads, head_tiles;  // query heads a key/value head, of which a block takes tile_heads in each of head_tiles
+    int heads_inverse;                  // ceil(2^16 / tile_heads): a tile's row r is token (r heads_inverse) >> 16 (exact below 2^16 / tile_heads rows)
+    FRY_DEVICE int token_of(int r) const { return (r * heads_inverse) >> 16; }
+    FRY_DEVICE int head_in_tile(int r) const { return r - token_of(r) * tile_heads; }
+    void set_tile(int rows) {  // as many query heads as a tile of `rows` rows takes
+        tile_heads = group < rows ? group : rows;
+        head_tiles = (group + tile_heads - 1) / tile_heads;
+        heads_inverse = (65536 + tile_heads - 1) / tile_heads;
+    }
     PackedRows queries;                 // packed; cached: count sequences of one row
     const int32_t* k_offsets;           // packed: [count + 1]
     int k_rows;

@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
     if (steps == 0) {  // no keys: zeros (or an empty split)
         for (int r = warp; r < 2 * kPromptTile; r += kPromptThreads / 32) {
-            const int token = r / kPromptTile * tile + r % kPromptTile / a.tile_heads, in_tile = head_tile * a.tile_heads + r % kPromptTile % a.tile_heads;
-            if (r % kPromptTile / a.tile_heads >= tile || token >= b.tokens || in_tile >= a.group) continue;
-            const AttentionOut to = attention_out(a, split, b.row + token, kv_head * a.group + in_tile);
+            const int row = r % kPromptTile, token = r / kPromptTile * tile + a.token_of(row), in_group = head_tile * a.tile_heads + a.head_in_tile(row);
+            if (a.token_of(row) >= tile || token >= b.tokens || in_group >= a.group) continue;
+            const AttentionOut to = attention_out(a, split, b.row + token, kv_head * a.group + in_group);
             if (a.splits > 1) {
                 if (lane == 0) to.part_sums[0] = -INFINITY, to.part_sums[1] = 0.0f;
             } else if (lane < a.width / 8) {
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegisters));
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // this thread's row of tile t
         const int count = counts[t];
-        const int token = t * tile + row / a.tile_heads, in_group = head_tile * a.tile_heads + row % a.tile_heads;
-        const bool live = row / a.tile_heads < tile && token < b.tokens && in_group < a.group;
+        const int token = t * tile + a.token_of(row), in_group = head_tile * a.tile_heads + a.head_in_tile(row);
+        const bool live = a.token_of(row) < tile && token < b.tokens && in_group < a.group;
         const int limit = live ? b.limit(token, a.causal) : INT_MAX;
         // the fewest keys a row of the warp sees: from there on scores are masked
         const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
@@ -381,8 +381,7 @@ bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int rank,
 template <int WIDTH, bool BF16>
 cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* error) {
     using S = PromptShape<WIDTH>;
-    a.tile_heads = a.group < kPromptTile ? a.group : kPromptTile;
-    a.head_tiles = (a.group + a.tile_heads - 1) / a.tile_heads;
+    a.set_tile(kPromptTile);
     const cuuint32_t tile = kPromptTile / a.tile_heads;
     using Dim = cuuint64_t;
     CUtensorMap map_q, map_k, map_v;
