@@ -7,6 +7,7 @@
 #include "../../include/fry_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "segments.cuh"
 
 namespace {
 
@@ -56,7 +57,7 @@ std::string attention_refusal(const fry::AttentionShape& s) {
     if (s.kv_heads <= 0 || s.heads <= 0 || s.heads > 1024 || s.heads % s.kv_heads != 0)
         return "takes 1 to 1024 query heads, a multiple of the key/value heads, got " + std::to_string(s.heads) + " and " + std::to_string(s.kv_heads);
     if (s.width <= 0 || s.width > 128 || s.width % 8 != 0) return "takes heads a multiple of 8 up to 128 wide, got " + std::to_string(s.width);
-    if (s.q_rows > (1 << 26) || s.sequences > (1 << 26)) return "takes up to 2^26 query rows and sequences";
+    if (s.q_rows > fry::kMaxPackedRows || s.sequences > fry::kMaxPackedRows) return "takes up to 2^24 - 1 query rows and sequences";
     return "";
 }
 
@@ -84,7 +85,7 @@ int run_attention(const char* name, const fry::AttentionShape& shape, const fry:
 // Why the adapters' kernels do not take a shape ("" if they do).
 std::string adapter_refusal(int kind, int M, int N, int K, int requests, int adapters, int rank) {
     const int k_unit = kind == 0 ? 16 : 8;
-    if (M < 0 || M > (1 << 24) || requests < 0 || requests > (1 << 24)) return "takes 0 to 2^24 rows and requests";
+    if (M < 0 || M > fry::kMaxPackedRows || requests < 0 || requests > fry::kMaxPackedRows) return "takes 0 to 2^24 - 1 rows and requests";
     if (N <= 0 || N % 8 != 0 || K <= 0 || K % k_unit != 0)
         return "takes N a multiple of 8 and K of " + std::to_string(k_unit) + ", got N " + std::to_string(N) + ", K " + std::to_string(K);
     if (rank <= 0 || rank % 8 != 0 || rank > 128) return "takes a rank of a multiple of 8 up to 128 (pad smaller ones with zeros), got " + std::to_string(rank);

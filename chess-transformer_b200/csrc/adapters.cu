@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kLowWarps * 32) adapter_low_kernel(const Adapt
     grid_dependency_start();
 
     const PackedRows rows{p.offsets, p.requests, M};
-    const int segment = find_segment(rows, p.tile_rows, slot, lane);
+    const int segment = find_segment(rows, TileRows(p.tile_rows), slot, lane);
     const int tile = slot - segment, tile_first = tile * p.tile_rows;
     const int first = max(rows.start(segment), tile_first), last = min(rows.start(segment + 1), min(M, tile_first + p.tile_rows));
     const bool request = segment >= 1 && segment <= p.requests;

@@ -141,6 +141,7 @@ constexpr int kMaxAttentionSplits = 64;
 enum class AttentionForm { kFew, kRows, kPrompt };
 struct AttentionPlan {
     AttentionForm form = AttentionForm::kRows;
+    int row_warps = 1;  // kRows: warps of 16 rows a block
     int splits = 1;
     size_t workspace_bytes = 0;
 };

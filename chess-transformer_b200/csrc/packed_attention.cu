@@ -22,39 +22,40 @@ FRY_DEVICE void cp_async16_or_zero(uint32_t shared, const void* global, bool rea
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(global), "r"(read ? 16 : 0) : "memory");
 }
 
-// WIDTH: the head width padded to 32, 64 or 128 with zeros. KEYS: the keys a warp takes of a stage (all of it with
-// ROW_WARPS, its own share with KEY_WARPS).
-template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES>
+// WIDTH: the head width padded to 32, 64 or 128 with zeros. KEY_WARPS: 1, the block's warps have 16 rows each and share the
+// keys; more, they have the same rows and KEYS keys each of a stage.
+constexpr int kMaxRowWarps = 8;
+template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES>
 struct RowsShape {
-    static_assert(ROW_WARPS == 1 || KEY_WARPS == 1, "warps share keys or rows");
-    static constexpr int kThreads = ROW_WARPS * KEY_WARPS * 32;
-    static constexpr int kRows = ROW_WARPS * 16;
+    static constexpr int kMaxThreads = (KEY_WARPS > 1 ? KEY_WARPS : kMaxRowWarps) * 32;
+    // blocks an SM: 8 warps of a narrow head in 64 registers a thread, 4 times over, hide the loads' latency
+    static constexpr int kBlocks = KEY_WARPS > 1 ? 1 : WIDTH == 32 ? 4 : WIDTH == 64 ? 2 : 1;
     static constexpr int kStageKeys = KEYS * KEY_WARPS;
     static constexpr int kTileBytes = kStageKeys * WIDTH * 2;  // the keys or the values of a stage
     static constexpr int kLoopBytes = STAGES * 2 * kTileBytes;
     // after the loop: a warp's 16 output rows, or with KEY_WARPS its 16 rows of fp32 sums, m and l
     static constexpr int kSumsPitch = WIDTH + 8;  // floats a row: the quads of a store in different banks
-    static constexpr int kJoinBytes = KEY_WARPS > 1 ? KEY_WARPS * 16 * (kSumsPitch + 2) * 4 : ROW_WARPS * 16 * WIDTH * 2;
-    static constexpr int kFoundAt = kLoopBytes > kJoinBytes ? kLoopBytes : kJoinBytes;  // the block's RowBlock
-    static constexpr int kSmemBytes = kFoundAt + 64;
+    __host__ __device__ static constexpr int join_bytes(int warps) { return KEY_WARPS > 1 ? KEY_WARPS * 16 * (kSumsPitch + 2) * 4 : warps * 16 * WIDTH * 2; }
+    __host__ __device__ static constexpr int found_at(int warps) { return kLoopBytes > join_bytes(warps) ? kLoopBytes : join_bytes(warps); }  // the block's RowBlock
+    static constexpr int smem_bytes(int warps) { return found_at(warps) + 64; }
     static_assert(sizeof(RowBlock) <= 64, "the block's rows fit their place");
 };
 
-template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
-__global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_kernel(const __grid_constant__ AttentionArgs a) {
-    using S = RowsShape<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES>;
+template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
+__global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kMaxThreads), (RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kBlocks))
+    attention_rows_kernel(const __grid_constant__ AttentionArgs a) {
+    using S = RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row_warp = KEY_WARPS > 1 ? 0 : warp, key_warp = KEY_WARPS > 1 ? warp : 0;
     grid_dependency_start();
     check_offsets(a);
 
-    const int tile = S::kRows / a.tile_heads;  // tokens a block
     // later tokens see more keys: they start first. One warp searches for all.
-    RowBlock* found = reinterpret_cast<RowBlock*>(smem + S::kFoundAt);
+    RowBlock* found = reinterpret_cast<RowBlock*>(smem + S::found_at(static_cast<int>(blockDim.x) / 32));
     if (warp == 0) {
         RowBlock mine;
-        if (!find_rows(a, tile, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, mine)) mine.tokens = 0;
+        if (!find_rows(a, a.slot_tokens, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, mine)) mine.tokens = 0;
         if (lane == 0) *found = mine;
     }
     __syncthreads();
@@ -83,18 +84,20 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         if (step < steps) {
             uint8_t* stage = smem + (step % STAGES) * 2 * S::kTileBytes;
             const uint32_t k_tile = smem_addr(stage), v_tile = k_tile + S::kTileBytes;
-            // each loader (the block, or a key warp for itself) copies KEYS rows
-            constexpr int kLoaders = KEY_WARPS > 1 ? 32 : S::kThreads;
-            const int me = KEY_WARPS > 1 ? lane : static_cast<int>(threadIdx.x), from = key_warp * KEYS;
-#pragma unroll
-            for (int i = 0; i < KEYS * kUnits / kLoaders; ++i) {
-                const int at = me + i * kLoaders, row = from + at / kUnits, unit = at % kUnits;
-                const int key = low + step * S::kStageKeys + row;
+            const int first = low + step * S::kStageKeys;
+            auto copy = [&](int row, int unit) {
+                const int key = first + row;
                 const bool read = key < high && unit < units;
                 cp_async16_or_zero(k_tile + tile_unit<WIDTH>(row, unit), keys + (read ? key * a.k_row + unit * 8 : 0), read);
                 cp_async16_or_zero(v_tile + tile_unit<WIDTH>(row, unit), values + (read ? key * a.v_row + unit * 8 : 0), read);
+            };
+            if constexpr (KEY_WARPS > 1) {  // a warp copies its own keys
+#pragma unroll
+                for (int i = 0; i < KEYS * kUnits / 32; ++i) copy(key_warp * KEYS + (lane + 32 * i) / kUnits, (lane + 32 * i) % kUnits);
+            } else {  // the block copies all, in whole 16s
+                const int rows = min(KEYS, (high - first + 15) / 16 * 16);
+                for (int at = threadIdx.x; at < rows * kUnits; at += blockDim.x) copy(at / kUnits, at % kUnits);
             }
-            static_assert(KEYS * kUnits % kLoaders == 0, "every thread copies the same number of units");
         }
         cp_async_commit();
     };
@@ -134,9 +137,9 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         else __syncthreads();
         load(step + STAGES - 1);  // into the stage read in the step before, which every reader has left
         const uint32_t k_tile = smem_addr(smem + (step % STAGES) * 2 * S::kTileBytes), v_tile = k_tile + S::kTileBytes;
-        if (idle) continue;
         const int first_key = low + step * S::kStageKeys + key_warp * KEYS, left = high - first_key;  // this warp's keys
-        float s[KEYS / 8][4] = {};
+        if (idle || left <= 0) continue;
+        float s[KEYS / 8][4];
         const uint32_t k_lane = k_tile + k_offset, v_lane = v_tile + v_offset;
 #pragma unroll
         for (int n = 0; n < KEYS / 16; ++n) {
@@ -145,6 +148,9 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
             for (int c = 0; c < WIDTH / 16; ++c) {
                 uint32_t f[4];
                 ldmatrix_x4(k_lane + n * 16 * WIDTH * 2 + k_units[c], f);
+                if (c == 0)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[2 * n][e] = s[2 * n + 1][e] = 0.0f;
                 mma16816<BF16>(s[2 * n], q[c], f[0], f[1]);
                 mma16816<BF16>(s[2 * n + 1], q[c], f[2], f[3]);
             }
@@ -250,17 +256,15 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
         }
     } else {
         uint8_t* staged = smem + warp * 16 * WIDTH * 2;
-        uint32_t again = 0;  // rows of the warp's 16 to compute again
+        bool finite[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int r = row_warp * 16 + g + 8 * half;
-            bool finite = true;
+            uint64_t zero2 = pair2(0.0f, 0.0f);  // 0 * o is 0 where o is finite, else NaN
 #pragma unroll
-            for (int c = 0; c < WIDTH / 8; ++c) finite = finite && isfinite(o[c][2 * half]) && isfinite(o[c][2 * half + 1]);
-            const uint32_t votes = __ballot_sync(0xffffffffu, !finite && isfinite(l[half]) && live(r));
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((votes >> (4 * i)) & 15u) again |= 1u << (8 * half + i);
+            for (int c = 0; c < WIDTH / 8; ++c) zero2 = fma2(pair2(o[c][2 * half], o[c][2 * half + 1]), pair2(0.0f, 0.0f), zero2);
+            const float2 zero = lanes(zero2);
+            finite[half] = zero.x + zero.y == 0.0f || !isfinite(l[half]) || !live(r);
             const float inverse = l[half] == 0.0f ? 0.0f : 1.0f / l[half];
             if (a.splits > 1) {
                 if (live(r)) {
@@ -288,8 +292,11 @@ __global__ void __launch_bounds__(ROW_WARPS * KEY_WARPS * 32) attention_rows_ker
             }
         }
         __syncwarp();
-        for (; again != 0; again &= again - 1) {
-            const int r = row_warp * 16 + __ffs(again) - 1, token = token_of(r);
+        if (__all_sync(0xffffffffu, finite[0] && finite[1])) return;
+        for (int i = 0; i < 16; ++i) {  // rows whose output is not finite though their sum is
+            const uint32_t votes = __ballot_sync(0xffffffffu, !finite[i / 8]);
+            if (((votes >> (i % 8 * 4)) & 15u) == 0) continue;
+            const int r = row_warp * 16 + i, token = token_of(r);
             recompute_row<BF16>(a, b, token, head_of(r), low, min(high, b.limit(token, a.causal)), split, lane);
         }
     }
@@ -341,30 +348,30 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
 
 namespace {
 
-template <int WIDTH, int ROW_WARPS, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
-cudaError_t launch_rows(AttentionArgs a, cudaStream_t stream) {
-    using S = RowsShape<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES>;
-    a.set_tile(S::kRows);
-    const int slots = a.lengths ? a.queries.count : packed_slots(a.queries.rows, S::kRows / a.tile_heads, a.queries.count);
-    auto kernel = attention_rows_kernel<WIDTH, ROW_WARPS, KEY_WARPS, KEYS, STAGES, BF16>;
-    const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
+template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES, bool BF16>
+cudaError_t launch_rows(AttentionArgs a, int row_warps, cudaStream_t stream) {
+    using S = RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>;
+    a.set_tile(row_warps * 16);
+    const int slots = a.lengths ? a.queries.count : packed_slots(a.queries.rows, a.slot_tokens.rows, a.queries.count);
+    const int warps = row_warps * KEY_WARPS, smem = S::smem_bytes(warps);
+    auto kernel = attention_rows_kernel<WIDTH, KEY_WARPS, KEYS, STAGES, BF16>;
+    const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
     if (status != cudaSuccess) return status;
-    return launch_dependent(kernel, dim3(slots, a.kv_heads * a.head_tiles, a.splits), dim3(S::kThreads), S::kSmemBytes, stream, a);
+    return launch_dependent(kernel, dim3(slots, a.kv_heads * a.head_tiles, a.splits), dim3(warps * 32), smem, stream, a);
 }
 
 template <int WIDTH, bool BF16>
-cudaError_t launch_width(const AttentionArgs& a, bool few, cudaStream_t stream) {
-    return few ? launch_rows<WIDTH, 1, 4, 16, 3, BF16>(a, stream) : launch_rows<WIDTH, 4, 1, 64, 2, BF16>(a, stream);
+cudaError_t launch_width(const AttentionArgs& a, const AttentionPlan& plan, cudaStream_t stream) {
+    return plan.form == AttentionForm::kFew ? launch_rows<WIDTH, 4, 16, 3, BF16>(a, 1, stream) : launch_rows<WIDTH, 1, 64, 2, BF16>(a, plan.row_warps, stream);
 }
 
 template <bool BF16>
-cudaError_t launch_type(const AttentionArgs& a, AttentionForm form, cudaStream_t stream, std::string* error) {
-    const bool few = form == AttentionForm::kFew;
+cudaError_t launch_type(const AttentionArgs& a, const AttentionPlan& plan, cudaStream_t stream, std::string* error) {
     cudaError_t status;
-    if (form == AttentionForm::kPrompt) status = a.width <= 64 ? launch_prompt<64, BF16>(a, stream, error) : launch_prompt<128, BF16>(a, stream, error);
-    else if (a.width <= 32) status = launch_width<32, BF16>(a, few, stream);
-    else if (a.width <= 64) status = launch_width<64, BF16>(a, few, stream);
-    else status = launch_width<128, BF16>(a, few, stream);
+    if (plan.form == AttentionForm::kPrompt) status = a.width <= 64 ? launch_prompt<64, BF16>(a, stream, error) : launch_prompt<128, BF16>(a, stream, error);
+    else if (a.width <= 32) status = launch_width<32, BF16>(a, plan, stream);
+    else if (a.width <= 64) status = launch_width<64, BF16>(a, plan, stream);
+    else status = launch_width<128, BF16>(a, plan, stream);
     if (status != cudaSuccess || a.splits == 1) return status;
     const int64_t count = static_cast<int64_t>(a.queries.rows) * a.heads;
     return launch_dependent(attention_join_kernel<BF16>, dim3(static_cast<unsigned>(count)), dim3(kJoinWarps * 32), 0, stream, a);
@@ -379,7 +386,13 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     const bool few = s.cached || mean_rows <= 16, prompt = !few && mean_rows >= 128 && mean_keys >= 128;
     plan.form = few ? AttentionForm::kFew : prompt ? AttentionForm::kPrompt : AttentionForm::kRows;
     // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
-    const int64_t group = s.heads / s.kv_heads, rows = few ? 16 : prompt ? 256 : 64, tile = rows / (group < rows ? group : rows);
+    const int64_t group = s.heads / s.kv_heads;
+    if (!few && !prompt) {
+        // a mean sequence's rows in as few blocks as take them, spread evenly
+        const int64_t row_blocks = (mean_rows + kMaxRowWarps * 16 - 1) / (kMaxRowWarps * 16);
+        plan.row_warps = static_cast<int>((mean_rows + row_blocks * 16 - 1) / (row_blocks * 16));
+    }
+    const int64_t rows = few ? 16 : prompt ? 256 : plan.row_warps * 16, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
     const int64_t wanted = (s.cached ? 16 : prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
@@ -391,7 +404,7 @@ AttentionPlan attention_plan(const AttentionShape& s) {
 
 cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors& x, float scale, void* workspace, cudaStream_t stream, std::string* error) {
     const AttentionPlan plan = attention_plan(shape);
-    AttentionArgs a = {};
+    AttentionArgs a;
     a.q = x.q, a.k = x.k, a.v = x.v, a.out = x.out;
     a.q_row = x.q_row, a.q_head = x.q_head, a.k_row = x.k_row, a.k_head = x.k_head, a.v_row = x.v_row, a.v_head = x.v_head;
     a.k_sequence = x.k_sequence, a.v_sequence = x.v_sequence;
@@ -404,7 +417,7 @@ cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors
     a.splits = plan.splits;
     a.part_sums = static_cast<float*>(workspace);
     a.part_out = a.part_sums + static_cast<size_t>(plan.splits) * shape.q_rows * shape.heads * 2;
-    return shape.bf16 ? launch_type<true>(a, plan.form, stream, error) : launch_type<false>(a, plan.form, stream, error);
+    return shape.bf16 ? launch_type<true>(a, plan, stream, error) : launch_type<false>(a, plan, stream, error);
 }
 
 }  // namespace fry

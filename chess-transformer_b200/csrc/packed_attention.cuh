@@ -31,30 +31,32 @@
 namespace fry {
 
 struct AttentionArgs {
-    const uint16_t *q, *k, *v;
-    uint16_t* out;                                         // [rows, heads, width] dense
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
-    int64_t k_sequence, v_sequence;                        // cached
-    int heads, kv_heads, width;
-    int group, tile_heads, head_tiles;  // query heads a key/value head, of which a block takes tile_heads in each of head_tiles
-    int heads_inverse;                  // ceil(2^16 / tile_heads): a tile's row r is token (r heads_inverse) >> 16 (exact below 2^16 / tile_heads rows)
+    const uint16_t *q = nullptr, *k = nullptr, *v = nullptr;
+    uint16_t* out = nullptr;                                         // [rows, heads, width] dense
+    int64_t q_row = 0, q_head = 0, k_row = 0, k_head = 0, v_row = 0, v_head = 0;  // strides in elements
+    int64_t k_sequence = 0, v_sequence = 0;                        // cached
+    int heads = 0, kv_heads = 0, width = 0;
+    int group = 1, tile_heads = 1, head_tiles = 1;  // query heads a key/value head, of which a block takes tile_heads in each of head_tiles
+    int heads_inverse = 0;                // ceil(2^16 / tile_heads): a tile's row r is token (r heads_inverse) >> 16 (exact below 2^16 / tile_heads rows)
     FRY_DEVICE int token_of(int r) const { return (r * heads_inverse) >> 16; }
     FRY_DEVICE int head_in_tile(int r) const { return r - token_of(r) * tile_heads; }
-    void set_tile(int rows) {  // as many query heads as a tile of `rows` rows takes
+    TileRows slot_tokens{1};            // the tokens of a slot
+    void set_tile(int rows, int tiles = 1) {  // as many query heads as a tile of `rows` rows takes, `tiles` tiles a slot
         tile_heads = group < rows ? group : rows;
         head_tiles = (group + tile_heads - 1) / tile_heads;
         heads_inverse = (65536 + tile_heads - 1) / tile_heads;
+        slot_tokens = TileRows(tiles * (rows / tile_heads));
     }
-    PackedRows queries;                 // packed; cached: count sequences of one row
-    const int32_t* k_offsets;           // packed: [count + 1]
-    int k_rows;
-    const int32_t* lengths;             // cached: [count], else null
-    int capacity;
-    int causal;
-    float scale_log2;                   // scale * log2(e), positive
-    int splits;
-    float* part_out;                    // [splits][rows][heads][width], where splits > 1
-    float* part_sums;                   // [splits][rows][heads][2]: m, l
+    PackedRows queries{};                // packed; cached: count sequences of one row
+    const int32_t* k_offsets = nullptr;          // packed: [count + 1]
+    int k_rows = 0;
+    const int32_t* lengths = nullptr;            // cached: [count], else null
+    int capacity = 0;
+    int causal = 0;
+    float scale_log2 = 0.0f;                 // scale * log2(e), positive
+    int splits = 1;
+    float* part_out = nullptr;                   // [splits][rows][heads][width], where splits > 1
+    float* part_sums = nullptr;                  // [splits][rows][heads][2]: m, l
 };
 
 // A block's rows: tokens [first, first + tokens) of a sequence of nq queries and nk keys.
@@ -71,7 +73,7 @@ struct RowBlock {
 };
 
 // The rows of block `slot` of tiles of `tile` tokens; false if it has none. Every thread of the warp calls it.
-FRY_DEVICE bool find_rows(const AttentionArgs& a, int tile, int slot, int lane, RowBlock& b) {
+FRY_DEVICE bool find_rows(const AttentionArgs& a, const TileRows& tile, int slot, int lane, RowBlock& b) {
     b.k_first = 0, b.k_base = b.v_base = 0;
     if (a.lengths) {
         if (slot >= a.queries.count) return false;
@@ -84,9 +86,9 @@ FRY_DEVICE bool find_rows(const AttentionArgs& a, int tile, int slot, int lane, 
     }
     const int segment = find_segment(a.queries, tile, slot, lane);
     const int start = a.queries.start(segment), end = a.queries.start(segment + 1);
-    b.first = (slot - start / tile - segment) * tile;
+    b.first = (slot - tile.of(start) - segment) * tile.rows;
     b.nq = end > start ? end - start : 0;
-    b.tokens = min(tile, b.nq - b.first);
+    b.tokens = min(tile.rows, b.nq - b.first);
     if (b.tokens <= 0) return false;
     b.row = start + b.first;
     b.nk = 0;

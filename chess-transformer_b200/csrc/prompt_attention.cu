@@ -113,12 +113,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     grid_dependency_start();
     check_offsets(a);
-    const int tile = kPromptTile / a.tile_heads;  // tokens a tile
+    const int tile = a.slot_tokens.rows / 2;  // tokens a tile
     RowBlock b;
     // later tokens see more keys: they start first
     const int at = blockIdx.x / (a.kv_heads * a.head_tiles), column = blockIdx.x % (a.kv_heads * a.head_tiles);
     const int slots = gridDim.x / (a.kv_heads * a.head_tiles);
-    if (!find_rows(a, 2 * tile, slots - 1 - at, lane, b)) return;  // uniform across the block
+    if (!find_rows(a, a.slot_tokens, slots - 1 - at, lane, b)) return;  // uniform across the block
     const int kv_head = column / a.head_tiles, head_tile = column % a.head_tiles;
     const int split = blockIdx.z;
     // keys of this split, in whole tiles; those a tile's last token sees
@@ -381,8 +381,8 @@ bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int rank,
 template <int WIDTH, bool BF16>
 cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* error) {
     using S = PromptShape<WIDTH>;
-    a.set_tile(kPromptTile);
-    const cuuint32_t tile = kPromptTile / a.tile_heads;
+    a.set_tile(kPromptTile, 2);
+    const cuuint32_t tile = a.slot_tokens.rows / 2;
     using Dim = cuuint64_t;
     CUtensorMap map_q, map_k, map_v;
     const Dim q_dims[4] = {Dim(a.width), Dim(a.group), Dim(a.queries.rows), Dim(a.kv_heads)};
@@ -396,7 +396,7 @@ cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* err
     auto kernel = attention_prompt_kernel<WIDTH, BF16>;
     const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
     if (status != cudaSuccess) return status;
-    const int slots = packed_slots(a.queries.rows, 2 * static_cast<int>(tile), a.queries.count);
+    const int slots = packed_slots(a.queries.rows, a.slot_tokens.rows, a.queries.count);
     return launch_dependent(kernel, dim3(slots * a.kv_heads * a.head_tiles, 1, a.splits), dim3(kPromptThreads), S::kSmemBytes, stream, map_q, map_k, map_v, a);
 }
 

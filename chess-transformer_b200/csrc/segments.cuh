@@ -22,6 +22,16 @@ struct PackedRows {
     }
 };
 
+// A tile's rows, and their division: row / rows is the high word of row * ceil(2^32 / rows), exact for row * rows < 2^32
+// (row * (ceil(2^32 / rows) * rows - 2^32) < 2^32), so up to kMaxPackedRows rows in tiles of up to 256.
+constexpr int kMaxPackedRows = (1 << 24) - 1;
+struct TileRows {
+    int rows;
+    uint32_t inverse;
+    __host__ __device__ explicit TileRows(int rows) : rows(rows), inverse(rows > 1 ? static_cast<uint32_t>(((1ull << 32) + rows - 1) / rows) : 0) {}
+    FRY_DEVICE int of(int row) const { return rows > 1 ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), inverse)) : row; }
+};
+
 // Slots. Segment i has the slots from start(i) / tile + i up to the next segment's: at least as many as its tiles of
 // `tile` rows, since start(i + 1) / tile - start(i) / tile + 1 >= ceil(length / tile), and at most one more. So a grid of
 // packed_slots(rows, tile, count) blocks holds every tile, and a block finds its segment by a search over the starts
@@ -30,11 +40,11 @@ __host__ __device__ inline int packed_slots(int rows, int tile, int count) { ret
 
 // The last segment i whose first slot is at most `slot`. The warp searches 32 ways at once: two steps up to 1024
 // requests. Every lane returns the same segment; for offsets that do not ascend it is some segment.
-FRY_DEVICE int find_segment(const PackedRows& packed, int tile, int slot, int lane) {
+FRY_DEVICE int find_segment(const PackedRows& packed, const TileRows& tile, int slot, int lane) {
     int low = 0, count = packed.count + 2;
     while (count > 1) {
         const int step = (count + 31) / 32, probe = lane * step;
-        const bool reached = probe < count && packed.start(low + probe) / tile + low + probe <= slot;
+        const bool reached = probe < count && tile.of(packed.start(low + probe)) + low + probe <= slot;
         const uint32_t votes = __ballot_sync(0xffffffffu, reached);
         const int last = votes == 0 ? 0 : 31 - __clz(votes);
         low += last * step;
