@@ -121,6 +121,7 @@ class _Library:
             if code != 0:
                 raise FryError(f"{name}: {self.handle.fry_last_error().decode(errors='replace')}")
             return code
+        setattr(self, name, checked)  # found at once from the next call on
         return checked
 
     def device_status(self, clear: bool = False) -> tuple[int, int]:

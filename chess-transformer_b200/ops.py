@@ -6,6 +6,7 @@ can be recorded in CUDA graphs and seen through by torch.compile (each has a fak
 refused with FryError: there is no CPU path.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -143,67 +144,86 @@ def _(q, k, v, heads):
     return torch.empty_like(q)
 
 
+# The packed operators below check a call in one expression and go on; where it does not hold, a second function finds out
+# what to say. A small call is bound by this host code (5.5 us of 13 are the library's, the rest torch's and Python's).
+
 def _call(function, index: int, *arguments) -> None:
     """A library call on device `index` and its current stream, whatever device is current."""
-    arguments += (torch._C._cuda_getCurrentRawStream(index),)
     if index == torch.cuda.current_device():
-        function(*arguments)
+        function(*arguments, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            function(*arguments)
+            function(*arguments, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _direct(x: torch.Tensor, *others: torch.Tensor | None) -> bool:
+def _direct(*tensors: torch.Tensor | None) -> bool:
     """Whether a call may skip torch's dispatcher (about 12 us of a small call): not under torch.compile, which must see
     the op, nor on fake tensors or where autograd would record it."""
-    if type(x) is not torch.Tensor or torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or type(tensors[0]) is not torch.Tensor:
         return False
-    return not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, *others))
+    return not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors)
 
 
-def _index32(name: str, tensor: torch.Tensor, what: str, count: int, device: torch.device) -> torch.Tensor:
+def _index32(name: str, tensor: torch.Tensor, what: str, count: int, device: torch.device) -> None:
     if tensor.dtype != torch.int32 or tensor.dim() != 1 or tensor.shape[0] != count or tensor.device != device:
         raise FryError(f"{name}: {what} must be int32 [{count}] on {device}, got {tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
-    return tensor.contiguous()
 
 
-def _strided(tensor: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
+def _readable(tensor: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
     """A 16-bit tensor as the attention kernels read it, its last axis dense and its other strides and its start on 16
-    bytes (a copy if they are not), and those strides."""
-    strides = [s if n > 1 else 8 for s, n in zip(tensor.stride()[:-1], tensor.shape)]
-    if (tensor.stride(-1) != 1 and tensor.shape[-1] > 1) or any(s % 8 or not s for s in strides) or tensor.data_ptr() % 16:
+    bytes (a copy if they are not), and those strides. An axis of one has no stride to keep."""
+    *strides, unit = tensor.stride()
+    if unit == 1 and not tensor.data_ptr() % 16 and all(s and not s % 8 for s in strides):
+        return tensor, strides
+    strides = [s if n > 1 else 8 for s, n in zip(strides, tensor.shape)]
+    if (unit != 1 and tensor.shape[-1] > 1) or any(s % 8 or not s for s in strides) or tensor.data_ptr() % 16:
         tensor = tensor.clone(memory_format=torch.contiguous_format)
         strides = [s if n > 1 else 8 for s, n in zip(tensor.stride()[:-1], tensor.shape)]
     return tensor, strides
 
 
-def _attention_types(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _refuse_attention(name: str, q, k, v, shaped: bool, indexes: dict, layout: str) -> None:
+    """Says what is wrong with a call of the attention ops."""
     _cuda(name, q, k, v)
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if q.dtype not in _HALVES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise FryError(f"{name}: q, k and v must be of one type, fp16 or bf16, got {q.dtype}, {k.dtype} and {v.dtype}")
     if k.device != q.device or v.device != q.device:
         raise FryError(f"{name}: q, k and v must be on one device, got {q.device}, {k.device} and {v.device}")
+    if shaped:
+        for what, (tensor, count) in indexes.items():
+            _index32(name, tensor, what, count, q.device)
+    raise FryError(f"{name} takes {layout}, heads a multiple of kv_heads, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(function: str, *shape: int) -> int:
+    return getattr(library(), function)(*shape)
 
 
 def _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale):
-    _attention_types("packed_attention", q, k, v)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2] or k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0:
-        raise FryError("packed_attention takes q [rows, heads, width] and k and v [key rows, kv_heads, width], heads a multiple of kv_heads, got "
-                       f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    if q_offsets.dim() != 1 or q_offsets.shape[0] < 1:
-        raise FryError(f"packed_attention: q_offsets must be int32 [sequences + 1], got {q_offsets.dtype} {tuple(q_offsets.shape)}")
-    count = q_offsets.shape[0]
-    q_offsets = _index32("packed_attention", q_offsets, "q_offsets", count, q.device)
-    k_offsets = _index32("packed_attention", k_offsets, "k_offsets", count, q.device)
-    (q, (q_row, q_head)), (k, (k_row, k_head)), (v, (v_row, v_head)) = _strided(q), _strided(k), _strided(v)
-    (rows, heads, width), (key_rows, kv_heads, _) = q.shape, k.shape
-    out = q.new_empty(rows, heads, width)
-    lib = library()
-    size = lib.fry_packed_attention_workspace_bytes(rows, key_rows, count - 1, heads, kv_heads, width)
+    q_shape, k_shape, dtype, index = q.shape, k.shape, q.dtype, q.get_device()
+    shaped = (len(q_shape) == 3 and len(k_shape) == 3 and v.shape == k_shape and q_shape[2] == k_shape[2] and k_shape[1] > 0
+              and q_shape[1] % k_shape[1] == 0)
+    if not (shaped and dtype in _HALVES and k.dtype is dtype and v.dtype is dtype and index >= 0
+            and k.get_device() == v.get_device() == q_offsets.get_device() == k_offsets.get_device() == index
+            and q_offsets.dtype is k_offsets.dtype is torch.int32 and q_offsets.dim() == 1 and q_offsets.shape == k_offsets.shape != (0,)):
+        count = max(q_offsets.numel(), 1)
+        _refuse_attention("packed_attention", q, k, v, shaped, {"q_offsets": (q_offsets, count), "k_offsets": (k_offsets, count)},
+                          "q [rows, heads, width] and k and v [key rows, kv_heads, width]")
+    (q, (q_row, q_head)), (k, (k_row, k_head)), (v, (v_row, v_head)) = _readable(q), _readable(k), _readable(v)
+    rows, heads, width = q_shape
+    key_rows, kv_heads, _ = k_shape
+    q_offsets, k_offsets = q_offsets.contiguous(), k_offsets.contiguous()
+    sequences = q_offsets.shape[0] - 1
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q_shape)
+    size = _workspace_bytes("fry_packed_attention_workspace_bytes", rows, key_rows, sequences, heads, kv_heads, width)
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
-    _call(lib.fry_packed_attention, q.device.index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
-          k_offsets.data_ptr(), rows, key_rows, count - 1, heads, kv_heads, width, q_row, q_head, k_row, k_head, v_row, v_head,
-          width ** -0.5 if scale is None else scale, causal, q.dtype == torch.bfloat16, workspace.data_ptr() if size else None, size)
+    _call(library().fry_packed_attention, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
+          k_offsets.data_ptr(), rows, key_rows, sequences, heads, kv_heads, width, q_row, q_head, k_row, k_head, v_row, v_head,
+          width ** -0.5 if scale is None else scale, causal, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
     return out
 
 
@@ -232,21 +252,23 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
 
 
 def _cached_attention(q, k, v, lengths, scale):
-    _attention_types("cached_attention", q, k, v)
-    if (q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[2] or k.shape[2] == 0
-            or q.shape[1] % k.shape[2] != 0):
-        raise FryError("cached_attention takes q [sequences, heads, width] and k and v [sequences, capacity, kv_heads, width], heads a multiple of "
-                       f"kv_heads, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    lengths = _index32("cached_attention", lengths, "lengths", q.shape[0], q.device)
-    (q, (q_row, q_head)), (k, (k_sequence, k_row, k_head)), (v, (v_sequence, v_row, v_head)) = _strided(q), _strided(k), _strided(v)
-    (sequences, heads, width), (_, capacity, kv_heads, _) = q.shape, k.shape
-    out = q.new_empty(sequences, heads, width)
-    lib = library()
-    size = lib.fry_cached_attention_workspace_bytes(sequences, capacity, heads, kv_heads, width)
+    q_shape, k_shape, dtype, index = q.shape, k.shape, q.dtype, q.get_device()
+    shaped = (len(q_shape) == 3 and len(k_shape) == 4 and v.shape == k_shape and k_shape[0] == q_shape[0] and q_shape[2] == k_shape[3]
+              and k_shape[2] > 0 and q_shape[1] % k_shape[2] == 0)
+    if not (shaped and dtype in _HALVES and k.dtype is dtype and v.dtype is dtype and index >= 0
+            and k.get_device() == v.get_device() == lengths.get_device() == index and lengths.dtype is torch.int32 and lengths.shape == q_shape[:1]):
+        _refuse_attention("cached_attention", q, k, v, shaped, {"lengths": (lengths, q_shape[0])},
+                          "q [sequences, heads, width] and k and v [sequences, capacity, kv_heads, width]")
+    (q, (q_row, q_head)), (k, (k_sequence, k_row, k_head)), (v, (v_sequence, v_row, v_head)) = _readable(q), _readable(k), _readable(v)
+    sequences, heads, width = q_shape
+    _, capacity, kv_heads, _ = k_shape
+    lengths = lengths.contiguous()
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q_shape)
+    size = _workspace_bytes("fry_cached_attention_workspace_bytes", sequences, capacity, heads, kv_heads, width)
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
-    _call(lib.fry_cached_attention, q.device.index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(), sequences,
+    _call(library().fry_cached_attention, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(), sequences,
           capacity, heads, kv_heads, width, q_row, q_head, k_sequence, k_row, k_head, v_sequence, v_row, v_head,
-          width ** -0.5 if scale is None else scale, q.dtype == torch.bfloat16, workspace.data_ptr() if size else None, size)
+          width ** -0.5 if scale is None else scale, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
     return out
 
 
@@ -274,15 +296,18 @@ def _aligned(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
 
 
-def _adapter_shapes(name: str, x, weight, bias, residual, down, up, offsets, ids) -> tuple[int, int, int, int, int, int]:
-    """(M, N, K, requests, adapters, rank) of a linear with adapters, or FryError."""
+def _refuse_adapters(name: str, x, weight, bias, residual, down, up, offsets, ids, dtype) -> None:
+    """Says what is wrong with a call of the linears with adapters."""
+    _cuda(name, x)
     for tensor in (weight, bias, residual, down, up, offsets, ids):
         if tensor is not None and tensor.device != x.device:
             raise FryError(f"{name}: x is on {x.device}, another operand on {tensor.device}")
+    _dtype(name, x, dtype, "x")
+    _dtype(name, weight, dtype, "weight")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise FryError(f"{name} takes x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
     N, K = weight.shape
-    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != K or up.shape[1] != N or up.shape[0] != down.shape[0] or up.shape[2] != down.shape[1]:
+    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != K or up.shape != (down.shape[0], N, down.shape[1]):
         raise FryError(f"{name} takes down [adapters, rank, {K}] and up [adapters, {N}, rank], got {tuple(down.shape)} and {tuple(up.shape)}")
     for tensor, what in ((bias, "bias"), (residual, "residual"), (down, "down"), (up, "up")):
         _dtype(name, tensor, torch.float16, what)
@@ -293,26 +318,33 @@ def _adapter_shapes(name: str, x, weight, bias, residual, down, up, offsets, ids
     requests = ids.shape[0] if ids.dim() == 1 else -1
     _index32(name, ids, "ids", requests, x.device)
     _index32(name, offsets, "offsets", requests + 1, x.device)
-    return x.numel() // K, N, K, requests, down.shape[0], down.shape[1]
+    raise FryError(f"{name}: cannot take this call")
 
 
-def _adapter_call(x, out, shapes, function, size, *operands):
-    """The library call of a linear with adapters into `out`: its operands' pointers, `out`, the sizes and a workspace."""
-    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
-    _call(function, x.device.index, *(None if t is None else t.data_ptr() for t in operands), out.data_ptr(), *shapes, workspace.data_ptr(), size)
-    return out
+def _adapter_operands(name: str, x, weight, bias, residual, down, up, offsets, ids, dtype) -> tuple[int, tuple[int, ...], tuple[torch.Tensor | None, ...]]:
+    """(device, (M, N, K, requests, adapters, rank), the operands dense and aligned) of a linear with adapters, or FryError."""
+    x_shape, w_shape, down_shape, index, half = x.shape, weight.shape, down.shape, x.get_device(), torch.float16
+    if not (index >= 0 and x.dtype is weight.dtype is dtype and down.dtype is up.dtype is half and offsets.dtype is ids.dtype is torch.int32
+            and len(w_shape) == 2 and len(x_shape) > 0 and x_shape[-1] == w_shape[1] and len(down_shape) == 3 and down_shape[2] == w_shape[1]
+            and up.shape == (down_shape[0], w_shape[0], down_shape[1]) and ids.dim() == 1 and offsets.shape == (ids.shape[0] + 1,)
+            and weight.get_device() == down.get_device() == up.get_device() == offsets.get_device() == ids.get_device() == index
+            and (bias is None or (bias.dtype is half and bias.shape == w_shape[:1] and bias.get_device() == index))
+            and (residual is None or (residual.dtype is half and residual.shape == (*x_shape[:-1], w_shape[0]) and residual.get_device() == index))):
+        _refuse_adapters(name, x, weight, bias, residual, down, up, offsets, ids, dtype)
+    N, K = w_shape
+    operands = (_aligned(x), _aligned(weight), bias if bias is None else bias.contiguous(), residual if residual is None else _aligned(residual),
+                _aligned(down), _aligned(up), offsets.contiguous(), ids.contiguous())
+    return index, (x.numel() // K if K else 0, N, K, ids.shape[0], down_shape[0], down_shape[1]), operands
 
 
 def _adapter_linear(x, weight, bias, residual, down, up, offsets, ids):
-    _cuda("adapter_linear", x)
-    _dtype("adapter_linear", x, torch.float16, "x")
-    _dtype("adapter_linear", weight, torch.float16, "weight")
-    shapes = _adapter_shapes("adapter_linear", x, weight, bias, residual, down, up, offsets, ids)
+    index, shapes, operands = _adapter_operands("adapter_linear", x, weight, bias, residual, down, up, offsets, ids, torch.float16)
     M, N, _, requests, _, rank = shapes
-    lib = library()
-    return _adapter_call(x, x.new_empty(*x.shape[:-1], N), shapes, lib.fry_adapter_linear, lib.fry_adapter_linear_workspace_bytes(M, N, requests, rank),
-                         _aligned(x), _aligned(weight), bias.contiguous() if bias is not None else None,
-                         _aligned(residual) if residual is not None else None, _aligned(down), _aligned(up), offsets.contiguous(), ids.contiguous())
+    out = x.new_empty(*x.shape[:-1], N)
+    size = _workspace_bytes("fry_adapter_linear_workspace_bytes", M, N, requests, rank)
+    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
+    _call(library().fry_adapter_linear, index, *(None if t is None else t.data_ptr() for t in operands), out.data_ptr(), *shapes, workspace.data_ptr(), size)
+    return out
 
 
 @torch.library.custom_op("fry::adapter_linear", mutates_args=())
@@ -339,20 +371,19 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
 
 def _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids):
     name = "int8_adapter_linear"
-    _cuda(name, x, x_scale, weight_scale)
-    _dtype(name, x, torch.int8, "x")
-    _dtype(name, weight, torch.int8, "weight")
-    shapes = _adapter_shapes(name, x, weight, bias, residual, down, up, offsets, ids)
+    index, shapes, (x, weight, *others) = _adapter_operands(name, x, weight, bias, residual, down, up, offsets, ids, torch.int8)
     M, N, _, requests, _, rank = shapes
-    _dtype(name, x_scale, torch.float32, "x_scale")
-    _dtype(name, weight_scale, torch.float32, "weight_scale")
-    if x_scale.numel() != M or weight_scale.numel() != N or x_scale.device != x.device or weight_scale.device != x.device:
-        raise FryError(f"{name} takes a scale a row of x and of weight on {x.device}, got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
-    lib = library()
+    if not (x_scale.dtype is weight_scale.dtype is torch.float32 and x_scale.numel() == M and weight_scale.numel() == N
+            and x_scale.get_device() == weight_scale.get_device() == index):
+        raise FryError(f"{name} takes an fp32 scale a row of x and of weight on {x.device}, got {x_scale.dtype} {tuple(x_scale.shape)} on "
+                       f"{x_scale.device} and {weight_scale.dtype} {tuple(weight_scale.shape)} on {weight_scale.device}")
+    x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
     out = x.new_empty(*x.shape[:-1], N, dtype=torch.float16)
-    return _adapter_call(x, out, shapes, lib.fry_int8_adapter_linear, lib.fry_int8_adapter_linear_workspace_bytes(M, N, requests, rank), _aligned(x),
-                         x_scale.contiguous(), _aligned(weight), weight_scale.contiguous(), bias.contiguous() if bias is not None else None,
-                         _aligned(residual) if residual is not None else None, _aligned(down), _aligned(up), offsets.contiguous(), ids.contiguous())
+    size = _workspace_bytes("fry_int8_adapter_linear_workspace_bytes", M, N, requests, rank)
+    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
+    _call(library().fry_int8_adapter_linear, index, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+          *(None if t is None else t.data_ptr() for t in others), out.data_ptr(), *shapes, workspace.data_ptr(), size)
+    return out
 
 
 @torch.library.custom_op("fry::int8_adapter_linear", mutates_args=())
