@@ -95,7 +95,7 @@ std::string adapter_refusal(int kind, int M, int N, int K, int requests, int ada
 
 size_t adapter_workspace_bytes(int kind, int M, int N, int requests, int rank) {
     if (M <= 0 || !adapter_refusal(kind, M, N, 16, requests, 1, rank).empty()) return 0;
-    return fry::AdapterWorkspace(M, requests, rank, fry::adapter_tile_rows(kind, M, N)).total;
+    return fry::AdapterWorkspace(kind, M, N, requests, rank).total;
 }
 
 int run_adapters(const char* name, int kind, fry::GemmArgs& args, fry::AdapterArgs& p, const void* weight, int M, int N, int K, void* workspace,

@@ -12,16 +12,17 @@
 // output costs too); its sums are fp32.
 #include "common.cuh"
 #include "kernels.h"
+#include "rowops.cuh"
 #include "segments.cuh"
 
 namespace fry {
 
-constexpr int kLowRows = 64, kLowWarps = 8;  // rows a block; its warps share 16-row groups and, beyond those, K
+constexpr int kThinRows = 64, kThinWarps = 8;  // rows of x a block takes; its warps share K
 
-// 16 bytes of x as fp16 pairs: 8 fp16 values, or 16 int8 values. int8 widens exactly: a byte with its sign bit flipped
-// in the low bits of 1024.0's fp16 pattern is 1024 + 128 + value.
+// 16 bytes as fp16 pairs: 8 fp16 values, or 16 int8 values. int8 widens exactly: a byte with its sign bit flipped in the
+// low bits of 1024.0's fp16 pattern is 1024 + 128 + value.
 template <bool INT8>
-FRY_DEVICE void low_pairs(const uint4& raw, uint32_t (&pairs)[INT8 ? 8 : 4]) {
+FRY_DEVICE void widen_pairs(const uint4& raw, uint32_t* pairs) {
     const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -40,17 +41,94 @@ FRY_DEVICE void low_pairs(const uint4& raw, uint32_t (&pairs)[INT8 ? 8 : 4]) {
     }
 }
 
-// TILES: 8-column tiles of the rank. A lane's MMA fragments come from 16-byte loads: of each run of K columns the four
-// lanes of a quad read 16 bytes each, and the MMA's K index is assigned to what a lane holds, alike for x and down (a sum
-// over K may take it in any order).
-template <bool INT8, int TILES>
-__global__ void __launch_bounds__(kLowWarps * 32) adapter_low_kernel(const AdapterArgs p, int M, int K) {
-    constexpr int kSteps = INT8 ? 4 : 2;          // MMA K steps of 16 a run
-    constexpr int kLane = kSteps * 4;             // K columns a lane holds of a run
+// A block's product of up to 64 rows of x, in `groups` of 16 (rows below `low` or from `high` on count as 0), with TILES * 8
+// rows of w (those from `columns` on count as 0), K long both: the warps take runs of K in turn and leave their sums in
+// partial [kThinWarps][64][TILES * 8]. A lane's MMA fragments come from 16-byte loads: of each run of K the four lanes of a
+// quad read 16 (of int8 x against fp16 w, 16 and 32) bytes each, and the MMA's K index is assigned to what a lane holds,
+// alike for x and w (a sum over K may take it in any order). Each block reads its x and w once, so the loads bound it.
+template <bool X_INT8, bool W_INT8, int TILES>
+FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
+    constexpr int kSteps = X_INT8 ? 4 : 2;          // MMA K steps of 16 a run
+    constexpr int kLane = kSteps * 4;               // K values a lane holds of a run
     constexpr int kRun = 4 * kLane;
-    extern __shared__ __align__(16) float partial[];  // [kLowWarps][16][TILES * 8]
+    constexpr int kGroups = kThinRows / 16, kLoads = X_INT8 && !W_INT8 ? 2 : 1;
+    constexpr int kAhead = TILES <= 2 ? 2 : 1;      // runs whose loads are in flight together
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int slot = blockIdx.x, part = blockIdx.y;
+    const uint8_t* x_lane = static_cast<const uint8_t*>(x) + (static_cast<size_t>(first_row + g) * K + t * kLane) * (X_INT8 ? 1 : 2);
+    const uint8_t* w_lane = static_cast<const uint8_t*>(w) + (static_cast<size_t>(g) * K + t * kLane) * (W_INT8 ? 1 : 2);
+    const size_t x_step = static_cast<size_t>(K) * 8 * (X_INT8 ? 1 : 2), w_step = static_cast<size_t>(K) * 8 * (W_INT8 ? 1 : 2);
+    float sums[kGroups][TILES][4] = {};
+    for (int run = warp * kRun; run < K; run += kThinWarps * kRun * kAhead) {
+        uint4 raw[kAhead][kGroups][2], weight[kAhead][TILES][kLoads];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = run + u * kThinWarps * kRun;
+            const bool inside = k + t * kLane < K;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int h = 0; h < kLoads; ++h)
+                    weight[u][n][h] = inside && n * 8 + g < columns
+                                          ? __ldg(reinterpret_cast<const uint4*>(w_lane + n * w_step + static_cast<size_t>(k) * (W_INT8 ? 1 : 2)) + h)
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int m = first_row + i * 16 + half * 8 + g;
+                    raw[u][i][half] = i < groups && inside && m >= low && m < high
+                                          ? *reinterpret_cast<const uint4*>(x_lane + (2 * i + half) * x_step + static_cast<size_t>(k) * (X_INT8 ? 1 : 2))
+                                          : make_uint4(0, 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            uint32_t b[TILES][2 * kSteps];
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int h = 0; h < kLoads; ++h) widen_pairs<W_INT8>(weight[u][n][h], b[n] + 4 * h);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                if (i >= groups) break;
+                uint32_t a[2][2 * kSteps];
+                widen_pairs<X_INT8>(raw[u][i][0], a[0]);
+                widen_pairs<X_INT8>(raw[u][i][1], a[1]);
+#pragma unroll
+                for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        mma_f16(sums[i][n], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[n][2 * s], b[n][2 * s + 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        if (i >= groups) break;
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                *reinterpret_cast<float2*>(partial + ((warp * kThinRows + i * 16 + half * 8 + g) * TILES + n) * 8 + 2 * t) =
+                    make_float2(sums[i][n][2 * half], sums[i][n][2 * half + 1]);
+    }
+}
+// The warps' sums of columns [column, column + COUNT) of a row, in the order of the warps.
+template <int TILES, int COUNT>
+FRY_DEVICE void thin_total(const float* partial, int row, int column, float (&total)[COUNT]) {
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) total[e] = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kThinWarps; ++q)
+#pragma unroll
+        for (int e = 0; e < COUNT; ++e) total[e] = __fadd_rn(total[e], partial[(q * kThinRows + row) * TILES * 8 + column + e]);
+}
+
+// low of 64 rows of a slot and up to TILES * 8 columns of the rank.
+template <bool INT8, int TILES>
+__global__ void __launch_bounds__(kThinWarps * 32) adapter_low_kernel(const AdapterArgs p, int M, int K) {
+    extern __shared__ __align__(16) float partial[];
+    const int lane = threadIdx.x & 31, slot = blockIdx.x, part = blockIdx.y, rank_first = blockIdx.z * TILES * 8;
     grid_dependency_start();
 
     const PackedRows rows{p.offsets, p.requests, M};
@@ -61,137 +139,156 @@ __global__ void __launch_bounds__(kLowWarps * 32) adapter_low_kernel(const Adapt
     int adapter = -1;
     if (request && first < last) adapter = p.ids[segment - 1];
     const bool known = adapter >= 0 && adapter < p.adapters;
-    if (slot == 0 && part == 0)  // one block records the requests that are not in range, for all
-        for (int s = threadIdx.x; s < p.requests; s += kLowWarps * 32)
-            if (rows.bad(s + 1) || p.ids[s] < -1 || p.ids[s] >= p.adapters) record_error(kBadOffsets, s);
-    if (part == 0 && threadIdx.x == 0) {
-        p.slot_adapter[slot] = known ? adapter : -1;
-        if (first < last && first == tile_first) p.tile_slots[tile].x = slot;
-        if (first < last && last == min(M, tile_first + p.tile_rows)) p.tile_slots[tile].y = slot + 1;
+    if (part == 0 && blockIdx.z == 0) {
+        if (slot == 0)  // one block records the requests that are not in range, for all
+            for (int s = threadIdx.x; s < p.requests; s += kThinWarps * 32)
+                if (rows.bad(s + 1) || p.ids[s] < -1 || p.ids[s] >= p.adapters) record_error(kBadOffsets, s);
+        if (p.row_slot)
+            for (int m = first + threadIdx.x; m < last; m += kThinWarps * 32) p.row_slot[m] = known ? slot : -1;
+        if (threadIdx.x == 0) {
+            p.slot_adapter[slot] = known ? adapter : -1;
+            if (first < last && first == tile_first) p.tile_slots[tile].x = slot;
+            if (first < last && last == min(M, tile_first + p.tile_rows)) p.tile_slots[tile].y = slot + 1;
+        }
     }
     if (!known) return;
 
-    const int part_first = tile_first + part * kLowRows;
-    const int low = max(first, part_first), high = min(last, part_first + kLowRows);  // this block's rows of the request
-    uint16_t* out = p.low + (static_cast<size_t>(slot) * p.tile_rows + part * kLowRows) * p.rank;
-    const int units = p.rank / 8;
-    if (low >= high) {
-        for (int i = threadIdx.x; i < kLowRows * units; i += kLowWarps * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    // the 16-row groups with rows of the request, and how many warps share each's K
-    const int group_first = (low - part_first) / 16, groups = (high - 1 - part_first) / 16 - group_first + 1;
-    const int shares = kLowWarps / groups, group = group_first + warp % groups, share = warp / groups;
-
-    float sums[TILES][4] = {};
-    if (share < shares) {
-        const uint8_t* x_rows[2];
-        bool mine[2];
+    const int part_first = tile_first + part * kThinRows, columns = min(TILES * 8, p.rank - rank_first), units = columns / 8;
+    const int low = max(first, part_first), high = min(last, part_first + kThinRows);  // this block's rows of the request
+    uint16_t* out = p.low + (static_cast<size_t>(slot) * p.tile_rows + part * kThinRows) * p.rank + rank_first;
+    if (low < high) {
+        // the 16-row groups from the first with a row of the request
+        const int group_first = (low - part_first) / 16, groups = (high - 1 - part_first) / 16 - group_first + 1;
+        thin_product<INT8, false, TILES>(p.x, part_first + group_first * 16, low, high, groups,
+                                         p.down + (static_cast<size_t>(adapter) * p.rank + rank_first) * K, columns, K, partial);
+        __syncthreads();
+        for (int i = threadIdx.x; i < kThinRows * units; i += kThinWarps * 32) {
+            const int row = i / units, unit = i % units, m = part_first + row;
+            uint4 packed = make_uint4(0, 0, 0, 0);
+            if (m >= low && m < high) {
+                float total[8];
+                thin_total<TILES>(partial, row - group_first * 16, unit * 8, total);
+                const float scale = INT8 ? p.x_scale[m] : 1.0f;
+                uint32_t* words = reinterpret_cast<uint32_t*>(&packed);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int m = part_first + group * 16 + g + 8 * half;
-            mine[half] = m >= low && m < high;
-            x_rows[half] = static_cast<const uint8_t*>(p.x) + static_cast<size_t>(mine[half] ? m : 0) * K * (INT8 ? 1 : 2);
-        }
-        const uint16_t* down = p.down + static_cast<size_t>(adapter) * p.rank * K;
-        constexpr int kAhead = TILES <= 4 ? 4 : 2;  // runs whose loads are in flight together
-        for (int run = share * kRun; run < K; run += shares * kRun * kAhead) {
-            uint4 raw[kAhead][2], weight[kAhead][TILES][INT8 ? 2 : 1];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int k = run + u * shares * kRun + t * kLane;
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                    raw[u][half] = k < K && mine[half] ? *reinterpret_cast<const uint4*>(x_rows[half] + static_cast<size_t>(k) * (INT8 ? 1 : 2)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int n = 0; n < TILES; ++n)
-#pragma unroll
-                    for (int h = 0; h < (INT8 ? 2 : 1); ++h)
-                        weight[u][n][h] = k < K && n < units ? *reinterpret_cast<const uint4*>(down + static_cast<size_t>(n * 8 + g) * K + k + 8 * h)
-                                                             : make_uint4(0, 0, 0, 0);
+                for (int e = 0; e < 4; ++e) words[e] = pack_half2_rn(__fmul_rn(total[2 * e], scale), __fmul_rn(total[2 * e + 1], scale));
             }
+            *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * p.rank + unit * 8) = packed;
+        }
+    } else {  // none of its rows: zeros
+        for (int i = threadIdx.x; i < kThinRows * units; i += kThinWarps * 32)
+            *reinterpret_cast<uint4*>(out + static_cast<size_t>(i / units) * p.rank + i % units * 8) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+// The whole linear for up to 64 rows, 16 columns a block: there its weights are read once and bound it, and the tensor
+// cores' 128-row tiles would be mostly empty (16 rows against 2048 x 2048 fp16 weights: 32 such tiles of 64 columns took
+// 15.8 us). Each block's product of x and its 16 weight rows is this kernel's; an output then adds low . up of its row's
+// adapter, rank products. The weights stream in while the kernel before this one still makes low.
+template <bool INT8>
+__global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const AdapterArgs p, const GemmArgs args, const void* weight, int M, int N, int K) {
+    constexpr int kTiles = 2, kColumns = kTiles * 8;
+    extern __shared__ __align__(16) float partial[];
+    const int slots = packed_slots(M, p.tile_rows, p.requests);
+    const int n0 = blockIdx.x * kColumns, columns = min(kColumns, N - n0);
+    thin_product<INT8, INT8, kTiles>(p.x, 0, 0, M, (M + 15) / 16, static_cast<const uint8_t*>(weight) + static_cast<size_t>(n0) * K * (INT8 ? 1 : 2), columns, K,
+                                     partial);
+    grid_dependency_start();  // low and row_slot are made
+    __syncthreads();
+    for (int i = threadIdx.x; i < M * kColumns / 2; i += kThinWarps * 32) {
+        const int m = i / (kColumns / 2), c = i % (kColumns / 2) * 2, n = n0 + c;
+        if (c >= columns) continue;
+        float total[2], added[2] = {0.0f, 0.0f};
+        thin_total<kTiles>(partial, m, c, total);
+        // (rows of offsets that descend may have no slot written)
+        const int slot = p.row_slot[m], adapter = slot >= 0 && slot < slots ? p.slot_adapter[slot] : -1;
+        if (adapter >= 0 && adapter < p.adapters) {
+            const uint4* low = reinterpret_cast<const uint4*>(p.low + (static_cast<size_t>(slot) * p.tile_rows + m % p.tile_rows) * p.rank);
+            const uint4* up = reinterpret_cast<const uint4*>(p.up + (static_cast<size_t>(adapter) * N + n) * p.rank);
+            for (int j = 0; j < p.rank / 8; ++j) {
+                float l[8], u[8];
+                unpack8(low[j], l);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                uint32_t a[2][INT8 ? 8 : 4];
-                low_pairs<INT8>(raw[u][0], a[0]);
-                low_pairs<INT8>(raw[u][1], a[1]);
+                for (int h = 0; h < 2; ++h) {
+                    unpack8(__ldg(up + h * (p.rank / 8) + j), u);
 #pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-                    const uint32_t* b = reinterpret_cast<const uint32_t*>(weight[u][n]);
-#pragma unroll
-                    for (int s = 0; s < kSteps; ++s) mma_f16(sums[n], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[2 * s], b[2 * s + 1]);
+                    for (int e = 0; e < 8; ++e) added[h] = __fmaf_rn(l[e], u[e], added[h]);
                 }
             }
         }
-    }
+        float value[2];
 #pragma unroll
-    for (int n = 0; n < TILES; ++n)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-            *reinterpret_cast<float2*>(partial + ((warp * 16 + g + 8 * half) * TILES + n) * 8 + 2 * t) = make_float2(sums[n][2 * half], sums[n][2 * half + 1]);
-    __syncthreads();
-    // the shares in order, scaled and rounded; rows of other requests 0
-    for (int i = threadIdx.x; i < kLowRows * units; i += kLowWarps * 32) {
-        const int row = i / units, unit = i % units, m = part_first + row;
-        uint4 packed = make_uint4(0, 0, 0, 0);
-        if (m >= low && m < high) {
-            const int from = row / 16 - group_first;
-            float values[8] = {};
-            for (int q = 0; q < shares; ++q) {
-                const float* source = partial + (((from + q * groups) * 16 + row % 16) * TILES + unit) * 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) values[e] = __fadd_rn(values[e], source[e]);
-            }
-            const float scale = INT8 ? p.x_scale[m] : 1.0f;
-            uint32_t* words = reinterpret_cast<uint32_t*>(&packed);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) words[e] = pack_half2_rn(__fmul_rn(values[2 * e], scale), __fmul_rn(values[2 * e + 1], scale));
+        for (int h = 0; h < 2; ++h) {
+            const float b = args.bias ? h2f_bits(args.bias[n + h]) : 0.0f;
+            // as the GEMM's epilogues: the scales and bias then the adapter (int8), or the adapter in the sums then the bias
+            value[h] = INT8 ? __fadd_rn(__fmaf_rn(__fmul_rn(total[h], args.x_scale[m]), args.w_scale[n + h], b), added[h])
+                            : __fadd_rn(__fadd_rn(total[h], added[h]), b);
         }
-        reinterpret_cast<uint4*>(out)[i] = packed;
+        const size_t at = static_cast<size_t>(m) * N + n;
+        if (args.residual) {
+            const __half2 residual = *reinterpret_cast<const __half2*>(args.residual + at);
+            value[0] = __fadd_rn(value[0], __low2float(residual)), value[1] = __fadd_rn(value[1], __high2float(residual));
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(args.out) + at) = pack_half2_rn(value[0], value[1]);
     }
 }
 
 namespace {
 
+constexpr int kThinMost = 32;  // rows up to which the thin kernel takes the linear
+
 template <bool INT8, int TILES>
 cudaError_t launch_low(const AdapterArgs& p, int M, int K, cudaStream_t stream) {
-    constexpr int kSmem = kLowWarps * 16 * TILES * 8 * 4;
+    constexpr int kSmem = kThinWarps * kThinRows * TILES * 8 * 4;
     auto kernel = adapter_low_kernel<INT8, TILES>;
     const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), kSmem);
     if (status != cudaSuccess) return status;
-    return launch_dependent(kernel, dim3(packed_slots(M, p.tile_rows, p.requests), p.tile_rows / kLowRows), dim3(kLowWarps * 32), kSmem, stream, p, M, K);
+    const dim3 grid(packed_slots(M, p.tile_rows, p.requests), (p.tile_rows + kThinRows - 1) / kThinRows, (p.rank + TILES * 8 - 1) / (TILES * 8));
+    return launch_dependent(kernel, grid, dim3(kThinWarps * 32), kSmem, stream, p, M, K);
 }
 
 template <bool INT8>
 cudaError_t low_rank_rows(const AdapterArgs& p, int M, int K, cudaStream_t stream) {
-    return p.rank <= 16   ? launch_low<INT8, 2>(p, M, K, stream)
+    return p.rank <= 8    ? launch_low<INT8, 1>(p, M, K, stream)
+           : p.rank <= 16 ? launch_low<INT8, 2>(p, M, K, stream)
            : p.rank <= 32 ? launch_low<INT8, 4>(p, M, K, stream)
-           : p.rank <= 64 ? launch_low<INT8, 8>(p, M, K, stream)
-                          : launch_low<INT8, 16>(p, M, K, stream);
+                          : launch_low<INT8, 8>(p, M, K, stream);
 }
+
+template <bool INT8>
+cudaError_t launch_thin(const AdapterArgs& p, const GemmArgs& args, const void* weight, int M, int N, int K, cudaStream_t stream) {
+    constexpr int kSmem = kThinWarps * kThinRows * 16 * 4;
+    return launch_dependent(adapter_thin_kernel<INT8>, dim3((N + 15) / 16), dim3(kThinWarps * 32), kSmem, stream, p, args, weight, M, N, K);
+}
+
+// the row tiles the slots are laid out by: the GEMM's, or of the thin kernel's rows all
+int slot_rows(int kind, int M, int N) { return M <= kThinMost ? kThinRows : adapter_tile_rows(kind, M, N); }
 
 }  // namespace
 
-// low [slots * tile_rows, rank] fp16, then tile_slots and slot_adapter, each 256-byte aligned
-AdapterWorkspace::AdapterWorkspace(int M, int requests, int rank, int tile_rows) {
-    const size_t slots = packed_slots(M, tile_rows, requests), tiles = (static_cast<size_t>(M) + tile_rows - 1) / tile_rows;
+AdapterWorkspace::AdapterWorkspace(int kind, int M, int N, int requests, int rank) : tile_rows(slot_rows(kind, M, N)) {
+    const size_t tiles = (static_cast<size_t>(M) + tile_rows - 1) / tile_rows;
     auto up = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    this->slots = slots;
+    slots = packed_slots(M, tile_rows, requests);
     tile_slots = up(slots * tile_rows * rank * 2);
     slot_adapter = tile_slots + up(tiles * sizeof(int2));
-    total = slot_adapter + up(slots * sizeof(int32_t));
+    row_slot = slot_adapter + up(slots * sizeof(int32_t));
+    total = row_slot + (M <= kThinMost ? up(M * sizeof(int32_t)) : 0);
 }
 
 cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& p, const void* weight, int M, int N, int K, void* workspace, cudaStream_t stream,
                            std::string* error) {
-    p.tile_rows = adapter_tile_rows(kind, M, N);
-    const AdapterWorkspace layout(M, p.requests, p.rank, p.tile_rows);
+    const AdapterWorkspace layout(kind, M, N, p.requests, p.rank);
     uint8_t* base = static_cast<uint8_t*>(workspace);
+    p.tile_rows = layout.tile_rows;
     p.low = reinterpret_cast<uint16_t*>(base);
     p.tile_slots = reinterpret_cast<int2*>(base + layout.tile_slots);
     p.slot_adapter = reinterpret_cast<int32_t*>(base + layout.slot_adapter);
+    const bool thin = M <= kThinMost;
+    if (thin) p.row_slot = reinterpret_cast<int32_t*>(base + layout.row_slot);
     const cudaError_t status = kind == 0 ? low_rank_rows<true>(p, M, K, stream) : low_rank_rows<false>(p, M, K, stream);
     if (status != cudaSuccess) return status;
+    if (thin) return kind == 0 ? launch_thin<true>(p, gemm_args, weight, M, N, K, stream) : launch_thin<false>(p, gemm_args, weight, M, N, K, stream);
     return adapter_gemm(kind, p, weight, gemm_args, static_cast<int>(layout.slots), M, N, K, stream, error);
 }
 

@@ -77,10 +77,13 @@ struct AdapterArgs {
     uint16_t* low = nullptr;
     int2* tile_slots = nullptr;
     int32_t* slot_adapter = nullptr;
+    int32_t* row_slot = nullptr;           // few rows: a row's slot (-1: no adapter)
 };
+// The workspace: low first, then the others where these say, each 256-byte aligned.
 struct AdapterWorkspace {
-    size_t slots, tile_slots, slot_adapter, total;
-    AdapterWorkspace(int M, int requests, int rank, int tile_rows);
+    int tile_rows;
+    size_t slots, tile_slots, slot_adapter, row_slot, total;
+    AdapterWorkspace(int kind, int M, int N, int requests, int rank);
 };
 int adapter_tile_rows(int kind, int M, int N);
 cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& adapters, const void* weight, int M, int N, int K, void* workspace,

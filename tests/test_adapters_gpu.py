@@ -95,6 +95,9 @@ SHAPES = [  # lengths, ids, adapters, rank, K, N
     ([64, 64, 128, 256, 512], [0, 1, 2, 3, -1], 4, 72, 128, 256),
     ([3000, 2500], [1, 0], 2, 32, 256, 2304),        # fp16: pairs of 256-row tiles
     ([37] * 150, [i % 11 - 1 for i in range(150)], 10, 40, 128, 2056),
+    ([1] * 32, [i % 20 - 1 for i in range(32)], 20, 16, 2048, 2040),
+    ([1] * 33, [i % 20 - 1 for i in range(33)], 20, 128, 1040, 264),
+    ([17, 0, 14], [1, 0, 1], 2, 64, 4096, 40),
     ([2] * 300, [i % 290 for i in range(300)], 290, 8, 64, 72),
 ]
 
@@ -107,7 +110,7 @@ def test_the_linear_with_adapters_is_its_definition(shape, bias, residual, int8)
 
 
 @pytest.mark.parametrize("int8", [False, True])
-@pytest.mark.parametrize("M", [90, 6000])
+@pytest.mark.parametrize("M", [2, 90, 6000])
 def test_rows_of_no_request_have_no_adapter(M, int8):
     Case(int8, [M, 7], [1, 0], 2, 16, 64, 2304, seed=20, first=13, behind=150).check()
     Case(int8, [], [], 2, 16, 64, 2304, seed=20, behind=M).check()
@@ -140,6 +143,18 @@ def test_an_adapter_reaches_its_own_requests_alone(N, bad, int8):
     assert not torch.isfinite(found[30:70, 5]).any() and not torch.isfinite(found[170:]).any()
     others = [c for c in range(N) if c != 5]
     assert ((found[30:70, others].double() - clean[0][30:70, others]).abs() <= clean[1][30:70, others]).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("int8", [False, True])
+def test_an_adapter_reaches_its_own_single_row_alone(int8, bad):
+    case = Case(int8, [1] * 9, [0, 1, -1] * 3, 2, 16, 64, 136, seed=33)
+    clean = case.expected()
+    case.up[1, 5, 3], case.down[1, 2, 1] = bad, bad
+    found = case.run()
+    others = [m for m in range(9) if m % 3 != 1]
+    assert ((found[others].double() - clean[0][others]).abs() <= clean[1][others]).all()
+    assert not torch.isfinite(found[1::3]).any()
 
 
 @pytest.mark.parametrize("int8", [False, True])
