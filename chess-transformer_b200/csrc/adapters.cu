@@ -46,20 +46,21 @@ FRY_DEVICE void widen_pairs(const uint4& raw, uint32_t* pairs) {
 // partial [kThinWarps][64][TILES * 8]. A lane's MMA fragments come from 16-byte loads: of each run of K the four lanes of a
 // quad read 16 (of int8 x against fp16 w, 16 and 32) bytes each, and the MMA's K index is assigned to what a lane holds,
 // alike for x and w (a sum over K may take it in any order). Each block reads its x and w once, so the loads bound it.
-template <bool X_INT8, bool W_INT8, int TILES>
-FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
+template <bool X_INT8, bool W_INT8, int TILES, int GROUPS>
+FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
     constexpr int kSteps = X_INT8 ? 4 : 2;          // MMA K steps of 16 a run
     constexpr int kLane = kSteps * 4;               // K values a lane holds of a run
     constexpr int kRun = 4 * kLane;
-    constexpr int kGroups = kThinRows / 16, kLoads = X_INT8 && !W_INT8 ? 2 : 1;
-    constexpr int kAhead = TILES <= 2 ? 2 : 1;      // runs whose loads are in flight together
+    constexpr int kLoads = X_INT8 && !W_INT8 ? 2 : 1;
+    // runs whose loads are in flight together: about 16 of 16 bytes a lane
+    constexpr int kPerRun = 2 * GROUPS + kLoads * TILES, kAhead = kPerRun <= 4 ? 4 : kPerRun <= 12 ? 2 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint8_t* x_lane = static_cast<const uint8_t*>(x) + (static_cast<size_t>(first_row + g) * K + t * kLane) * (X_INT8 ? 1 : 2);
     const uint8_t* w_lane = static_cast<const uint8_t*>(w) + (static_cast<size_t>(g) * K + t * kLane) * (W_INT8 ? 1 : 2);
     const size_t x_step = static_cast<size_t>(K) * 8 * (X_INT8 ? 1 : 2), w_step = static_cast<size_t>(K) * 8 * (W_INT8 ? 1 : 2);
-    float sums[kGroups][TILES][4] = {};
+    float sums[GROUPS][TILES][4] = {};
     for (int run = warp * kRun; run < K; run += kThinWarps * kRun * kAhead) {
-        uint4 raw[kAhead][kGroups][2], weight[kAhead][TILES][kLoads];
+        uint4 raw[kAhead][GROUPS][2], weight[kAhead][TILES][kLoads];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int k = run + u * kThinWarps * kRun;
@@ -72,7 +73,7 @@ FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, in
                                           ? __ldg(reinterpret_cast<const uint4*>(w_lane + n * w_step + static_cast<size_t>(k) * (W_INT8 ? 1 : 2)) + h)
                                           : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i)
+            for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int m = first_row + i * 16 + half * 8 + g;
@@ -89,7 +90,7 @@ FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, in
 #pragma unroll
                 for (int h = 0; h < kLoads; ++h) widen_pairs<W_INT8>(weight[u][n][h], b[n] + 4 * h);
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
+            for (int i = 0; i < GROUPS; ++i) {
                 if (i >= groups) break;
                 uint32_t a[2][2 * kSteps];
                 widen_pairs<X_INT8>(raw[u][i][0], a[0]);
@@ -103,7 +104,7 @@ FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, in
         }
     }
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
         if (i >= groups) break;
 #pragma unroll
         for (int n = 0; n < TILES; ++n)
@@ -112,6 +113,11 @@ FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, in
                 *reinterpret_cast<float2*>(partial + ((warp * kThinRows + i * 16 + half * 8 + g) * TILES + n) * 8 + 2 * t) =
                     make_float2(sums[i][n][2 * half], sums[i][n][2 * half + 1]);
     }
+}
+template <bool X_INT8, bool W_INT8, int TILES>
+FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
+    if (groups == 1) thin_product_of<X_INT8, W_INT8, TILES, 1>(x, first_row, low, high, 1, w, columns, K, partial);
+    else thin_product_of<X_INT8, W_INT8, TILES, kThinRows / 16>(x, first_row, low, high, groups, w, columns, K, partial);
 }
 // The warps' sums of columns [column, column + COUNT) of a row, in the order of the warps.
 template <int TILES, int COUNT>
@@ -126,7 +132,7 @@ FRY_DEVICE void thin_total(const float* partial, int row, int column, float (&to
 
 // low of 64 rows of a slot and up to TILES * 8 columns of the rank.
 template <bool INT8, int TILES>
-__global__ void __launch_bounds__(kThinWarps * 32) adapter_low_kernel(const AdapterArgs p, int M, int K) {
+__global__ void __launch_bounds__(kThinWarps * 32, TILES <= 2 ? 2 : 1) adapter_low_kernel(const AdapterArgs p, int M, int K) {
     extern __shared__ __align__(16) float partial[];
     const int lane = threadIdx.x & 31, slot = blockIdx.x, part = blockIdx.y, rank_first = blockIdx.z * TILES * 8;
     grid_dependency_start();
