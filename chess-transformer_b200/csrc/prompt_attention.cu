@@ -7,15 +7,17 @@
 // 4-7 are the softmax of the two tiles, a thread a row. The tiles alternate: while one tile's scores are on the softmax,
 // the tensor core works on the other's, P V of its last keys and then Q K^T of its next ones.
 //
-// TMEM (512 columns of 32 bits): S0, S1 (128 columns each), O0, O1 (WIDTH each). A tile's P, two 16-bit values a column,
-// overwrites the first half of its S, which the thread that writes it has read; the next Q K^T into S follows P V, and one
-// thread issues both, so the tensor core takes them in order. Its commit is also what tells the softmax that the P V
-// before it is done and O may be touched.
+// TMEM (512 columns of 32 bits): S0, S1 (128 columns each), O0, O1 (WIDTH each) and P0, P1 (64 each: two 16-bit values a
+// column). At width 128 that is 128 columns too many: there a tile's P overwrites the first half of its S, which the thread
+// that writes it has read, and the next Q K^T into S follows P V; one thread issues both, and products of one shape are
+// taken in the order they are issued in. At width 64 the two have different shapes, whose order is not defined, but P has
+// columns of its own: the next Q K^T is issued as soon as the softmax has read S, and P waits for the P V before it.
 //
-// Softmax: a row's 128 scores are in its thread's registers, so maximum and sum need no exchange. The running maximum m may
-// lag behind: as long as no row of the warp has risen by more than 2^8 the probabilities are taken against the old m (they
-// stay below 2^8, exact in the same relative steps) and O is left as it is; only then O is read, scaled and written back.
-// The first tile of keys always sets m, so the largest probability of a row is at least 1.
+// Softmax: a row's 128 scores are in its thread's registers, so maximum and sum need no exchange, and P V of the first 64
+// starts while the thread is at the others. The running maximum m may lag behind: the first probabilities are taken
+// against the m of the keys before, while the new maximum is still being found, and as long as no row of the warp has risen
+// by more than 2^8 they stand (they stay below 2^8, in the same relative steps); only where one has, O and the sum are
+// scaled to the new m. The first tile of keys always sets m, so the largest probability of a row is at least 1.
 #include "common.cuh"
 #include "kernels.h"
 #include "packed_attention.cuh"
@@ -36,6 +38,10 @@ struct PromptShape {
     static constexpr int kStages = WIDTH == 128 ? 5 : 8;    // key and value tiles in turn
     static constexpr int kBarrierBytes = 256;
     static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + kBarrierBytes;
+    // TMEM columns
+    static constexpr bool kShared = WIDTH == 128;             // P lies in S
+    static constexpr int kOutAt = 2 * kPromptTile, kProbabilitiesAt = kShared ? 0 : kOutAt + 2 * WIDTH, kProbabilities = kShared ? kPromptTile : 64;
+    static_assert(kShared || kProbabilitiesAt + 2 * kProbabilities <= 512, "TMEM holds P beside S and O");
     static_assert(kSmemBytes <= 227 * 1024, "the queries, the stages and the barriers fit");
 };
 
@@ -98,16 +104,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     uint64_t* q_full = reinterpret_cast<uint64_t*>(stages + S::kStages * S::kTileBytes);
     uint64_t* full = q_full + 1;                          // [kStages]
     uint64_t* empty = full + S::kStages;                  // [kStages]
-    uint64_t* s_full = empty + S::kStages;                // [2]: a tile's scores are there, and its last P V is done
-    uint64_t* p_full = s_full + 2;                        // [2][2]: the first and second half of its probabilities are
-    uint64_t* o_full = p_full + 4;                        // [2]: its output is
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+    uint64_t* s_full = empty + S::kStages;                // [2]: a tile's scores are there
+    uint64_t* s_read = s_full + 2;                        // [2]: they have been read (width 64)
+    uint64_t* p_full = s_read + 2;                        // [2][2]: the first and second half of its probabilities are there
+    uint64_t* pv_done = p_full + 4;                       // [2]: P V is done
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < S::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&o_full[t], 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_read[t], kPromptSoftmaxWarps / 2), mbar_init(&pv_done[t], 1);
         for (int h = 0; h < 4; ++h) mbar_init(&p_full[h], kPromptSoftmaxWarps / 2);
         fence_barrier_init();
     }
@@ -181,12 +188,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 constexpr uint32_t score_desc = prompt_desc<BF16>(kPromptTile, false), out_desc = prompt_desc<BF16>(WIDTH, true);
                 auto stage = [&](int i) { return smem_addr(stages + (i % S::kStages) * S::kTileBytes); };
                 auto wait_stage = [&](int i) { return mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, 32); };
+                // an address's 16-byte units are a descriptor's low bits: steps are added to it
                 auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
-                    const uint32_t q = smem_addr(queries + t * S::kTileBytes), k = stage(2 * j);
+                    const uint64_t q = smem_desc_sw128(smem_addr(queries + t * S::kTileBytes)), k = smem_desc_sw128(stage(2 * j));
 #pragma unroll
                     for (int c = 0; c < WIDTH / 16; ++c) {
-                        const uint32_t offset = (c / 4) * S::kBoxBytes + (c % 4) * 32;
-                        mma_ss<1>(tmem + t * kPromptTile, smem_desc_sw128(q + offset), smem_desc_sw128(k + offset), score_desc, c > 0 ? 1u : 0u);
+                        const int units = ((c / 4) * S::kBoxBytes + (c % 4) * 32) / 16;
+                        mma_ss<1>(tmem + t * kPromptTile, q + units, k + units, score_desc, c > 0 ? 1u : 0u);
                     }
                     mma_commit(&s_full[t]);
                 };
@@ -199,26 +207,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 }
                 for (int j = 0; j < steps && ok; ++j) {
                     const int v_stage = 2 * j + 1, k_next = 2 * j + 2;
-                    ok = wait_stage(v_stage) && (j + 1 >= steps || wait_stage(k_next));
+                    if (j + 1 < steps) ok = wait_stage(k_next);
+                    if constexpr (!S::kShared) {
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            if (j + 1 >= counts[t]) continue;
+                            ok = mbar_wait(&s_read[t], j & 1, 39);
+                            tc_fence_after();
+                            if (ok) scores(t, j + 1);
+                        }
+                        if (j + 1 < steps) mma_commit(&empty[k_next % S::kStages]);
+                    }
+                    ok = ok && wait_stage(v_stage);
+                    const uint64_t v = value_desc(stage(v_stage));
                     for (int t = 0; t < 2 && ok; ++t) {
                         if (j >= counts[t]) continue;
                         // O_t += P_t V_j over the keys the tile sees, 16 an MMA, in the halves that P comes in
                         const int keys = min(kPromptTile, highs[t] - low - j * kPromptTile), chunks = (keys + 15) / 16;
+                        const uint32_t o = tmem + S::kOutAt + t * WIDTH, p = tmem + S::kProbabilitiesAt + t * S::kProbabilities;
                         for (int half = 0; half < 2 && ok; ++half) {
                             ok = mbar_wait(&p_full[2 * t + half], j & 1, 34);
                             if (!ok) break;
                             tc_fence_after();
-                            for (int c = 4 * half; c < min(chunks, 4 * half + 4); ++c)
-                                mma_ts(tmem + 2 * kPromptTile + t * WIDTH, tmem + t * kPromptTile + c * 8, value_desc(stage(v_stage) + c * 16 * 128), out_desc,
-                                       j > 0 || c > 0 ? 1u : 0u);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int c = 4 * half + i;
+                                if (c < chunks) mma_ts(o, p + c * 8, v + c * 16 * 128 / 16, out_desc, j > 0 || c > 0 ? 1u : 0u);
+                            }
                         }
                         if (!ok) break;
-                        if (j + 1 < counts[t]) scores(t, j + 1);
-                        else mma_commit(&o_full[t]);
+                        mma_commit(&pv_done[t]);
+                        if (S::kShared && j + 1 < counts[t]) scores(t, j + 1);
                     }
                     if (ok) {
                         mma_commit(&empty[v_stage % S::kStages]);
-                        if (j + 1 < steps) mma_commit(&empty[k_next % S::kStages]);
+                        if (S::kShared && j + 1 < steps) mma_commit(&empty[k_next % S::kStages]);
                     }
                 }
             }
@@ -229,89 +251,110 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int count = counts[t];
         const int token = t * tile + a.token_of(row), in_group = head_tile * a.tile_heads + a.head_in_tile(row);
         const bool live = a.token_of(row) < tile && token < b.tokens && in_group < a.group;
-        const int limit = live ? b.limit(token, a.causal) : INT_MAX;
+        const int limit = min(b.nk, live ? b.limit(token, a.causal) : INT_MAX);
         // the fewest keys a row of the warp sees: from there on scores are masked
         const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
         const uint32_t lanes_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_tmem = tmem + t * kPromptTile + lanes_at, o_tmem = tmem + 2 * kPromptTile + t * WIDTH + lanes_at;
+        const uint32_t s_tmem = tmem + t * kPromptTile + lanes_at, o_tmem = tmem + S::kOutAt + t * WIDTH + lanes_at;
+        const uint32_t p_tmem = tmem + S::kProbabilitiesAt + t * S::kProbabilities + lanes_at;
+        const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
         float m = -INFINITY;
         uint64_t totals[2] = {pair2(0.0f, 0.0f), pair2(0.0f, 0.0f)};
         bool alive = true;
         for (int j = 0; j < count; ++j) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, 35))) {
-                alive = false;
-                break;
-            }
+            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, 35));
+            if (!alive) break;
             tc_fence_after();
             const int first_key = low + j * kPromptTile;
             uint32_t raw[4][32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_load32(s_tmem + c * 32, raw[c]);
             tmem_load_wait();
-            if (first_key + kPromptTile > min(warp_limit, b.nk)) {
-                const int here = min(limit, b.nk) - first_key;
+            if constexpr (!S::kShared) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_read[t]);
+                __syncwarp();
+            }
+            if (first_key + kPromptTile > warp_limit) {
+                const int here = limit - first_key;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (c * 32 + e >= here) raw[c][e] = __float_as_uint(-INFINITY);
             }
-            float top[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                top[c] = fmaxf(__uint_as_float(raw[c][0]), __uint_as_float(raw[c][1]));
-#pragma unroll
-                for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]));
-            }
-            const float risen = fmaxf(m, max3(top[0], top[1], fmaxf(top[2], top[3])) * a.scale_log2);
-            if (__any_sync(0xffffffffu, risen > m + kLagLog2)) {
-                const float shrink = ex2_approx_ftz(m - (risen == -INFINITY ? 0.0f : risen));
-                const uint64_t shrink2 = pair2(shrink, shrink);
-                m = risen;
-                totals[0] = mul2(totals[0], shrink2), totals[1] = mul2(totals[1], shrink2);
-                if (j > 0) {  // O is complete up to the keys before these
-#pragma unroll 1
-                    for (int c = 0; c < WIDTH; c += 32) {
-                        uint32_t o[32];
-                        tmem_load32(o_tmem + c, o);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-                        tmem_store32(o_tmem + c, o);
-                    }
-                }
-            }
             // value rows behind the sequence's last key that the last MMA's 16 keys still take are another sequence's: zeros
             if (first_key + kPromptTile > b.nk && (highs[t] - first_key + 15) / 16 * 16 > b.nk - first_key) {
                 const int i = 2 * j + 1;
-                if (!__all_sync(0xffffffffu, mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, 36))) alive = false;
+                alive = __all_sync(0xffffffffu, mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, 36));
                 uint8_t* values = stages + (i % S::kStages) * S::kTileBytes;
                 const int from = b.nk - first_key, rows = 16 - b.nk % 16;
                 for (int u = threadIdx.x & 127; u < rows * (WIDTH / 8) && alive; u += 128)
                     *reinterpret_cast<uint4*>(values + (u % (WIDTH / 8)) / 8 * S::kBoxBytes + (from + u / (WIDTH / 8)) * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_shared();
+                __syncwarp();
             }
-            const float base = m == -INFINITY ? 0.0f : -m;
-            const uint64_t base2 = pair2(base, base), scale2 = pair2(a.scale_log2, a.scale_log2);
+            auto highest = [&] {
+                float top[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t packed[32];
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = fmaxf(__uint_as_float(raw[c][0]), __uint_as_float(raw[c][1]));
+#pragma unroll
+                    for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]));
+                }
+                return fmaxf(m, max3(top[0], top[1], fmaxf(top[2], top[3])) * a.scale_log2);
+            };
+            uint32_t packed[32];
+            uint64_t sums[2];
+            auto probabilities = [&](int half) {  // of 64 keys, and their sums
+                const float base = m == -INFINITY ? 0.0f : -m;
+                const uint64_t base2 = pair2(base, base);
+                sums[0] = sums[1] = pair2(0.0f, 0.0f);
 #pragma unroll
                 for (int e = 0; e < 64; e += 2) {
                     const uint32_t* from = &raw[half * 2 + e / 32][e % 32];
                     const float2 x = lanes(fma2(pair2(__uint_as_float(from[0]), __uint_as_float(from[1])), scale2, base2));
                     const float2 p = make_float2(ex2_approx_ftz(x.x), ex2_approx_ftz(x.y));
-                    totals[e / 2 % 2] = add2(totals[e / 2 % 2], pair2(p.x, p.y));
+                    sums[e / 2 % 2] = add2(sums[e / 2 % 2], pair2(p.x, p.y));
                     packed[e / 2] = pack16<BF16>(p.x, p.y);
                 }
-                tmem_store32(s_tmem + half * 32, packed);
+            };
+            auto hand_over = [&](int half) {  // to the MMAs
+                totals[0] = add2(totals[0], sums[0]), totals[1] = add2(totals[1], sums[1]);
+                tmem_store32(p_tmem + half * 32, packed);
                 tmem_store_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
+                __syncwarp();  // together again before the next warp-wide TMEM access
+            };
+            if (j == 0) m = highest();
+            probabilities(0);
+            const float risen = highest();
+            // P V of the keys before is done: at width 128 the scores came after it
+            if (!S::kShared && j > 0) alive = __all_sync(0xffffffffu, alive && mbar_wait(&pv_done[t], (j - 1) & 1, 38));
+            if (__any_sync(0xffffffffu, risen > m + kLagLog2)) {
+                const float shrink = risen == -INFINITY ? 0.0f : ex2_approx_ftz(m - risen);
+                m = risen;
+                totals[0] = mul2(totals[0], pair2(shrink, shrink)), totals[1] = mul2(totals[1], pair2(shrink, shrink));
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_tmem + c, o);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                    tmem_store32(o_tmem + c, o);
+                }
+                probabilities(0);
             }
+            hand_over(0);
+            probabilities(1);
+            hand_over(1);
         }
-        if (count > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, 37));
+        if (count > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (count - 1) & 1, 37));
         tc_fence_after();
         const float2 both = lanes(add2(totals[0], totals[1]));
         const float total = both.x + both.y, inverse = total == 0.0f ? 0.0f : 1.0f / total;
