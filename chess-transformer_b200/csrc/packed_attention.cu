@@ -51,11 +51,11 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
     grid_dependency_start();
     check_offsets(a);
 
-    // later tokens see more keys: they start first. One warp searches for all.
+    // one warp searches for all
     RowBlock* found = reinterpret_cast<RowBlock*>(smem + S::found_at(static_cast<int>(blockDim.x) / 32));
     if (warp == 0) {
         RowBlock mine;
-        if (!find_rows(a, a.slot_tokens, static_cast<int>(gridDim.x - 1 - blockIdx.x), lane, mine)) mine.tokens = 0;
+        if (!find_rows(a, a.slot_tokens, blockIdx.x, lane, mine)) mine.tokens = 0;
         if (lane == 0) *found = mine;
     }
     __syncthreads();
@@ -321,12 +321,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
     const float top = warp_max(fmaxf(mine[0].x, mine[1].x)), base = top == -INFINITY ? 0.0f : top;
     float total = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+    const int column = 4 * lane < a.width ? lane : 0;
+#pragma unroll 8
     for (int s = warp; s < a.splits; s += kJoinWarps) {
-        const float m = __shfl_sync(0xffffffffu, s < 32 ? mine[0].x : mine[1].x, s & 31), l = __shfl_sync(0xffffffffu, s < 32 ? mine[0].y : mine[1].y, s & 31);
+        float4 part = reinterpret_cast<const float4*>(a.part_out + (s * count + at) * a.width)[column];
+        const float2 sums = s < 32 ? mine[0] : mine[1];
+        const float m = __shfl_sync(0xffffffffu, sums.x, s & 31), l = __shfl_sync(0xffffffffu, sums.y, s & 31);
         const float share = ex2_approx_ftz(m - base);
-        float4 part = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a split without keys for this row has written no output
-        if (l != 0.0f && 4 * lane < a.width) part = reinterpret_cast<const float4*>(a.part_out + (s * count + at) * a.width)[lane];
+        if (l == 0.0f) part = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a split without keys for this row may have written none
         total = __fmaf_rn(share, l, total);
         o.x = __fmaf_rn(share, part.x, o.x), o.y = __fmaf_rn(share, part.y, o.y), o.z = __fmaf_rn(share, part.z, o.z), o.w = __fmaf_rn(share, part.w, o.w);
     }
@@ -394,7 +396,8 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     }
     const int64_t rows = few ? 16 : prompt ? 256 : plan.row_warps * 16, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
-    const int64_t wanted = (s.cached ? 16 : prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    // (a cache's: a block an SM where that splits every sequence, else sixteen, which even out their lengths)
+    const int64_t wanted = (s.cached && blocks >= kSms ? 16 : few || prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
     const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;
@@ -415,8 +418,8 @@ cudaError_t packed_attention(const AttentionShape& shape, const AttentionTensors
     a.causal = shape.causal;
     a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
     a.splits = plan.splits;
-    a.part_sums = static_cast<float*>(workspace);
-    a.part_out = a.part_sums + static_cast<size_t>(plan.splits) * shape.q_rows * shape.heads * 2;
+    a.part_out = static_cast<float*>(workspace);  // first: it is read 16 bytes at a time
+    a.part_sums = a.part_out + static_cast<size_t>(plan.splits) * shape.q_rows * shape.heads * shape.width;
     return shape.bf16 ? launch_type<true>(a, plan, stream, error) : launch_type<false>(a, plan, stream, error);
 }
 

@@ -86,9 +86,10 @@ FRY_DEVICE bool find_rows(const AttentionArgs& a, const TileRows& tile, int slot
     }
     const int segment = find_segment(a.queries, tile, slot, lane);
     const int start = a.queries.start(segment), end = a.queries.start(segment + 1);
-    b.first = (slot - tile.of(start) - segment) * tile.rows;
     b.nq = end > start ? end - start : 0;
-    b.tokens = min(tile.rows, b.nq - b.first);
+    // a sequence's last tile first: later tokens see more keys, and the longest work is best started early
+    b.first = ((b.nq + tile.rows - 1) / tile.rows - 1 - (slot - tile.of(start) - segment)) * tile.rows;
+    b.tokens = b.first < 0 ? 0 : min(tile.rows, b.nq - b.first);
     if (b.tokens <= 0) return false;
     b.row = start + b.first;
     b.nk = 0;
@@ -101,10 +102,10 @@ FRY_DEVICE bool find_rows(const AttentionArgs& a, const TileRows& tile, int slot
     return true;
 }
 
-// Records a sequence whose offsets descend or leave their tensor. One block of a launch does it for all, the first: it has
+// Records a sequence whose offsets descend or leave their tensor. One block of a launch does it for all, the last: it has
 // the rows behind the last sequence, usually none.
 FRY_DEVICE void check_offsets(const AttentionArgs& a) {
-    if (a.lengths || blockIdx.x != 0 || blockIdx.y != 0 || blockIdx.z != 0) return;
+    if (a.lengths || blockIdx.x != gridDim.x - 1 || blockIdx.y != 0 || blockIdx.z != 0) return;
     const PackedRows keys{a.k_offsets, a.queries.count, a.k_rows};
     for (int s = threadIdx.x; s < a.queries.count; s += blockDim.x)
         if (a.queries.bad(s + 1) || keys.bad(s + 1)) record_error(kBadOffsets, s);

@@ -122,10 +122,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     check_offsets(a);
     const int tile = a.slot_tokens.rows / 2;  // tokens a tile
     RowBlock b;
-    // later tokens see more keys: they start first
     const int at = blockIdx.x / (a.kv_heads * a.head_tiles), column = blockIdx.x % (a.kv_heads * a.head_tiles);
-    const int slots = gridDim.x / (a.kv_heads * a.head_tiles);
-    if (!find_rows(a, a.slot_tokens, slots - 1 - at, lane, b)) return;  // uniform across the block
+    if (!find_rows(a, a.slot_tokens, at, lane, b)) return;  // uniform across the block
     const int kv_head = column / a.head_tiles, head_tile = column % a.head_tiles;
     const int split = blockIdx.z;
     // keys of this split, in whole tiles; those a tile's last token sees

@@ -91,6 +91,8 @@ SHAPES = [  # queries, keys (None: the queries' own), heads, kv_heads, width
     ([300], None, 130, 1, 8),                         # 130 of them
     ([700, 513], None, 4, 1, 128),
     ([400], [1500], 6, 2, 128),
+    ([1], [900], 1, 1, 24),          # 3 splits of one row: the partial results' places are odd
+    ([3, 1, 1], [700, 800, 900], 1, 1, 128),
 ]
 
 
@@ -193,6 +195,8 @@ CACHES = [  # lengths, capacity, heads, kv_heads, width
     ([64] * 40, 64, 8, 8, 24),
     ([20000, 3], 20000, 16, 2, 128),
     ([600] * 50, 640, 4, 4, 128),
+    ([900], 900, 1, 1, 40),          # 3 splits of one row: the partial results' places are odd
+    ([1300, 7, 5], 1300, 3, 1, 8),
 ]
 
 
