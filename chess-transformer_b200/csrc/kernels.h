@@ -144,7 +144,8 @@ constexpr int kMaxAttentionSplits = 64;
 enum class AttentionForm { kFew, kRows, kPrompt };
 struct AttentionPlan {
     AttentionForm form = AttentionForm::kRows;
-    int row_warps = 1;  // kRows: warps of 16 rows a block
+    int row_warps = 1;       // kRows: warps of 16 rows a block
+    bool long_keys = false;  // kPrompt: two tiles a block
     int splits = 1;
     size_t workspace_bytes = 0;
 };

@@ -370,7 +370,9 @@ cudaError_t launch_width(const AttentionArgs& a, const AttentionPlan& plan, cuda
 template <bool BF16>
 cudaError_t launch_type(const AttentionArgs& a, const AttentionPlan& plan, cudaStream_t stream, std::string* error) {
     cudaError_t status;
-    if (plan.form == AttentionForm::kPrompt) status = a.width <= 64 ? launch_prompt<64, BF16>(a, stream, error) : launch_prompt<128, BF16>(a, stream, error);
+    if (plan.form == AttentionForm::kPrompt && a.width <= 64) status = launch_prompt<64, 1, BF16>(a, stream, error);
+    else if (plan.form == AttentionForm::kPrompt && plan.long_keys) status = launch_prompt<128, 2, BF16>(a, stream, error);
+    else if (plan.form == AttentionForm::kPrompt) status = launch_prompt<128, 1, BF16>(a, stream, error);
     else if (a.width <= 32) status = launch_width<32, BF16>(a, plan, stream);
     else if (a.width <= 64) status = launch_width<64, BF16>(a, plan, stream);
     else status = launch_width<128, BF16>(a, plan, stream);
@@ -394,10 +396,11 @@ AttentionPlan attention_plan(const AttentionShape& s) {
         const int64_t row_blocks = (mean_rows + kMaxRowWarps * 16 - 1) / (kMaxRowWarps * 16);
         plan.row_warps = static_cast<int>((mean_rows + row_blocks * 16 - 1) / (row_blocks * 16));
     }
-    const int64_t rows = few ? 16 : prompt ? 256 : plan.row_warps * 16, tile = rows / (group < rows ? group : rows);
+    plan.long_keys = prompt && s.width > 64 && mean_keys >= 6144;  // two tiles a block (prompt_attention.cu)
+    const int64_t rows = few ? 16 : prompt ? (plan.long_keys ? 256 : 128) : plan.row_warps * 16, tile = rows / (group < rows ? group : rows);
     const int64_t blocks = s.kv_heads * ((group + rows - 1) / rows) * (s.cached ? sequences : (s.q_rows + tile - 1) / tile + sequences / 2);
     // (a cache's: a block an SM where that splits every sequence, else sixteen, which even out their lengths)
-    const int64_t wanted = (s.cached && blocks >= kSms ? 16 : few || prompt ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
+    const int64_t wanted = (s.cached && blocks >= kSms ? 16 : few || plan.long_keys ? 1 : 2) * kSms / (blocks > 0 ? blocks : 1), most = mean_keys / 256;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxAttentionSplits ? kMaxAttentionSplits : splits);
     const size_t parts = static_cast<size_t>(plan.splits) * s.q_rows * s.heads;

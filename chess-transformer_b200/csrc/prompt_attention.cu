@@ -1,17 +1,26 @@
 // Attention over packed sequences on the fifth-generation tensor cores, for sequences of many rows (packed_attention.cu has
 // the operator's definition, the other kernels and the choice between them).
 //
-// A block takes two tiles of 128 rows (a row is a token and one of the query heads that share its keys) against keys in
+// A block takes TILES tiles of 128 rows (a row is a token and one of the query heads that share its keys) against keys in
 // tiles of 128, each of the products a tcgen05.mma of M = 128: scores S = Q K^T into TMEM, and O += P V with P read from
-// TMEM. Warp 8 streams the key and value tiles through a ring of stages with TMA, warp 9 issues the MMAs, and warps 0-3 and
-// 4-7 are the softmax of the two tiles, a thread a row. The tiles alternate: while one tile's scores are on the softmax,
-// the tensor core works on the other's, P V of its last keys and then Q K^T of its next ones.
+// TMEM. One warp streams the key and value tiles through a ring of stages with TMA, one issues the MMAs, and four warps a
+// tile are its softmax, a thread a row. Two tiles are on an SM, so that while one's scores are on the softmax the tensor
+// core works on the other's products: in two blocks of one, or in one block of two.
+// Two blocks start and end on their own, one's beginning and end under the other's work; one block's tiles share its key
+// and value stages, half the traffic from L2. Measured (two blocks / one): 8 x 512 tokens of 12 heads of 64 after ragged
+// keys 46.5 / 58.5 us, 16 prompts of 1000 tokens, 32 heads of 128, 232 / 244 us, one of 4096 151 / 154 us, of 8192 503 / 482 us.
+// What bounds it: a step of both tiles (2 x 128 rows by 128 keys) takes about 3400 clocks at width 128, of which the
+// tensor core is busy for 2048 and the exponentials (16 a clock and SM) for 2048. A row tile's chain of loads from TMEM
+// (250 clocks), exponentials (64 at a time 520 to 900, with the other tile at its own), hand-over and products (1100)
+// does not fill either; splitting S in two steps of 64 keys so that the softmax never waits loses more to the narrower
+// products (their operands' shared memory reads bound them), exponentials in part on the FMA pipe gained 1%, two warps a
+// row or turns at the exponentials lost 10 to 25%.
 //
-// TMEM (512 columns of 32 bits): S0, S1 (128 columns each), O0, O1 (WIDTH each) and P0, P1 (64 each: two 16-bit values a
-// column). At width 128 that is 128 columns too many: there a tile's P overwrites the first half of its S, which the thread
-// that writes it has read, and the next Q K^T into S follows P V; one thread issues both, and products of one shape are
-// taken in the order they are issued in. At width 64 the two have different shapes, whose order is not defined, but P has
-// columns of its own: the next Q K^T is issued as soon as the softmax has read S, and P waits for the P V before it.
+// TMEM (512 columns of 32 bits an SM): a tile's S (128 columns), O (WIDTH) and P (64: two 16-bit values a column). At width
+// 128 that is 64 columns too many: there P overwrites the first half of S, which the thread that writes it has read, and
+// the next Q K^T into S follows P V; one thread issues both, and products of one shape are taken in the order they are
+// issued in. At width 64 the two have different shapes, whose order is not defined, but P has columns of its own: the next
+// Q K^T is issued as soon as the softmax has read S, and P waits for the P V before it.
 //
 // Softmax: a row's 128 scores are in its thread's registers, so maximum and sum need no exchange, and P V of the first 64
 // starts while the thread is at the others. The running maximum m may lag behind: the first probabilities are taken
@@ -24,25 +33,28 @@
 
 namespace fry {
 
-constexpr int kPromptTile = 128;                // rows of a tile, and keys of a stage
-constexpr int kPromptSoftmaxWarps = 8, kPromptLoadWarp = 8, kPromptMmaWarp = 9, kPromptThreads = 12 * 32;
-// Registers a thread: the launch gives 168 to each of the three groups of four warps (384 threads x 168 = 64512); the
-// softmax's two groups take 208, which hold a row's 128 scores, the third keeps 88 (2 x 128 x 208 + 128 x 88 = 64512).
-constexpr int kPromptSoftmaxRegisters = 208, kPromptOtherRegisters = 88;
+constexpr int kPromptTile = 128;  // rows of a tile, and keys of a stage
 constexpr float kLagLog2 = 8.0f;
 
-template <int WIDTH>
+template <int WIDTH, int TILES>
 struct PromptShape {
+    static constexpr int kBlocks = 2 / TILES;               // blocks an SM
     static constexpr int kBoxBytes = kPromptTile * 128;     // 128 rows of 64 columns, the 128-byte swizzle
     static constexpr int kTileBytes = WIDTH / 64 * kBoxBytes;
-    static constexpr int kStages = WIDTH == 128 ? 5 : 8;    // key and value tiles in turn
-    static constexpr int kBarrierBytes = 256;
-    static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + kBarrierBytes;
+    static constexpr int kStages = TILES == 2 ? 5 : WIDTH == 128 ? 2 : 4;  // key and value tiles in turn
+    static constexpr int kBarrierBytes = 512;
+    static constexpr int kSmemBytes = (TILES + kStages) * kTileBytes + kBarrierBytes;
+    // warps: the tiles' softmax, then a group of four of which the first loads and the second issues the MMAs
+    static constexpr int kSoftmaxWarps = 4 * TILES, kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1, kThreads = (kSoftmaxWarps + 4) * 32;
+    // Registers a thread: the softmax's warps take 208, which hold a row's 128 scores, and leave the others what remains of
+    // the launch's: 168 a thread of 384 (256 x 208 + 128 x 88 = 64512), 128 of 256 (128 x 208 + 128 x 48 = 32768).
+    static constexpr int kSoftmaxRegisters = 208, kOtherRegisters = TILES == 2 ? 88 : 48;
     // TMEM columns
-    static constexpr bool kShared = WIDTH == 128;             // P lies in S
-    static constexpr int kOutAt = 2 * kPromptTile, kProbabilitiesAt = kShared ? 0 : kOutAt + 2 * WIDTH, kProbabilities = kShared ? kPromptTile : 64;
-    static_assert(kShared || kProbabilitiesAt + 2 * kProbabilities <= 512, "TMEM holds P beside S and O");
-    static_assert(kSmemBytes <= 227 * 1024, "the queries, the stages and the barriers fit");
+    static constexpr bool kShared = WIDTH == 128;           // P lies in S
+    static constexpr int kOutAt = TILES * kPromptTile, kProbabilitiesAt = kShared ? 0 : kOutAt + TILES * WIDTH, kProbabilities = kShared ? kPromptTile : 64;
+    static constexpr int kColumns = TILES * 256;
+    static_assert(kBlocks * (kSmemBytes + 1024) <= 228 * 1024, "an SM holds the blocks");
+    static_assert(TILES * (kPromptTile + WIDTH + (kShared ? 0 : 64)) <= kColumns, "TMEM holds the tiles");
 };
 
 // D[tmem] (+)= A[tmem] * B[smem], 16-bit A two values a column
@@ -89,18 +101,18 @@ __host__ __device__ constexpr uint32_t prompt_desc(int n, bool rows_are_k) {
     return instr_desc<1>(n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (rows_are_k ? 1u << 16 : 0u);
 }
 
-template <int WIDTH, bool BF16>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+template <int WIDTH, int TILES, bool BF16>
+__global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (PromptShape<WIDTH, TILES>::kBlocks))
     attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttentionArgs a) {
-    using S = PromptShape<WIDTH>;
+    using S = PromptShape<WIDTH, TILES>;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_addr(smem) & 1023u) {  // uniform across the block
         if (threadIdx.x == 0) record_error(kMisaligned, 30);
         return;
     }
     uint8_t* queries = smem;                              // [2][boxes][128 rows][128 bytes]
-    uint8_t* stages = smem + 2 * S::kTileBytes;           // [kStages][boxes][128 keys][128 bytes]
+    uint8_t* stages = smem + TILES * S::kTileBytes;           // [kStages][boxes][128 keys][128 bytes]
     uint64_t* q_full = reinterpret_cast<uint64_t*>(stages + S::kStages * S::kTileBytes);
     uint64_t* full = q_full + 1;                          // [kStages]
     uint64_t* empty = full + S::kStages;                  // [kStages]
@@ -114,13 +126,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < S::kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_read[t], kPromptSoftmaxWarps / 2), mbar_init(&pv_done[t], 1);
-        for (int h = 0; h < 4; ++h) mbar_init(&p_full[h], kPromptSoftmaxWarps / 2);
+        for (int t = 0; t < TILES; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_read[t], 4), mbar_init(&pv_done[t], 1);
+        for (int h = 0; h < 4; ++h) mbar_init(&p_full[h], 4);
         fence_barrier_init();
     }
     grid_dependency_start();
     check_offsets(a);
-    const int tile = a.slot_tokens.rows / 2;  // tokens a tile
+    const int tile = a.slot_tokens.rows / TILES;  // tokens a tile
     RowBlock b;
     const int at = blockIdx.x / (a.kv_heads * a.head_tiles), column = blockIdx.x % (a.kv_heads * a.head_tiles);
     if (!find_rows(a, a.slot_tokens, at, lane, b)) return;  // uniform across the block
@@ -134,12 +146,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int tokens = min(b.tokens - t * tile, tile);
         return tokens <= 0 ? low : max(low, min(high, b.limit(t * tile + tokens - 1, a.causal)));
     };
-    const int highs[2] = {tile_high(0), tile_high(1)};
+    const int highs[2] = {tile_high(0), TILES > 1 ? tile_high(1) : low};
     auto count_of = [&](int t) { return (highs[t] - low + kPromptTile - 1) / kPromptTile; };
     const int counts[2] = {count_of(0), count_of(1)}, steps = max(counts[0], counts[1]);
 
     if (steps == 0) {  // no keys: zeros (or an empty split)
-        for (int r = warp; r < 2 * kPromptTile; r += kPromptThreads / 32) {
+        for (int r = warp; r < TILES * kPromptTile; r += S::kThreads / 32) {
             const int row = r % kPromptTile, token = r / kPromptTile * tile + a.token_of(row), in_group = head_tile * a.tile_heads + a.head_in_tile(row);
             if (a.token_of(row) >= tile || token >= b.tokens || in_group >= a.group) continue;
             const AttentionOut to = attention_out(a, split, b.row + token, kv_head * a.group + in_group);
@@ -151,8 +163,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         return;
     }
-    if (warp == kPromptMmaWarp) {
-        tmem_alloc(tmem_slot, 512);
+    if (warp == S::kMmaWarp) {
+        tmem_alloc(tmem_slot, S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -160,9 +172,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp >= kPromptSoftmaxWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegisters));
-        if (warp == kPromptLoadWarp) {
+    if (warp >= S::kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
+        if (warp == S::kLoadWarp) {
             if (elect_one()) {
                 const int tiles = counts[1] > 0 ? 2 : 1;
                 // a box has whole tokens: tile * tile_heads rows of the 128
@@ -181,7 +193,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                                     b.k_first + low + (i >> 1) * kPromptTile, kv_head);
                 }
             }
-        } else if (warp == kPromptMmaWarp) {
+        } else if (warp == S::kMmaWarp) {
             if (elect_one()) {
                 constexpr uint32_t score_desc = prompt_desc<BF16>(kPromptTile, false), out_desc = prompt_desc<BF16>(WIDTH, true);
                 auto stage = [&](int i) { return smem_addr(stages + (i % S::kStages) * S::kTileBytes); };
@@ -199,7 +211,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 bool ok = mbar_wait(q_full, 0, 33) && wait_stage(0);
                 tc_fence_after();
                 if (ok) {
-                    for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < TILES; ++t)
                         if (counts[t] > 0) scores(t, 0);
                     mma_commit(&empty[0]);
                 }
@@ -207,7 +219,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const int v_stage = 2 * j + 1, k_next = 2 * j + 2;
                     if (j + 1 < steps) ok = wait_stage(k_next);
                     if constexpr (!S::kShared) {
-                        for (int t = 0; t < 2 && ok; ++t) {
+                        for (int t = 0; t < TILES && ok; ++t) {
                             if (j + 1 >= counts[t]) continue;
                             ok = mbar_wait(&s_read[t], j & 1, 39);
                             tc_fence_after();
@@ -217,7 +229,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                     ok = ok && wait_stage(v_stage);
                     const uint64_t v = value_desc(stage(v_stage));
-                    for (int t = 0; t < 2 && ok; ++t) {
+                    for (int t = 0; t < TILES && ok; ++t) {
                         if (j >= counts[t]) continue;
                         // O_t += P_t V_j over the keys the tile sees, 16 an MMA, in the halves that P comes in
                         const int keys = min(kPromptTile, highs[t] - low - j * kPromptTile), chunks = (keys + 15) / 16;
@@ -244,8 +256,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegisters));
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // this thread's row of tile t
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegisters));
+        const int t = TILES > 1 ? warp >> 2 : 0, row = (warp & 3) * 32 + lane;  // this thread's row of tile t
         const int count = counts[t];
         const int token = t * tile + a.token_of(row), in_group = head_tile * a.tile_heads + a.head_in_tile(row);
         const bool live = a.token_of(row) < tile && token < b.tokens && in_group < a.group;
@@ -399,9 +411,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kPromptMmaWarp) {
+    if (warp == S::kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, S::kColumns);
     }
 }
 
@@ -419,11 +431,11 @@ bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int rank,
     return result == CUDA_SUCCESS;
 }
 
-template <int WIDTH, bool BF16>
+template <int WIDTH, int TILES, bool BF16>
 cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* error) {
-    using S = PromptShape<WIDTH>;
-    a.set_tile(kPromptTile, 2);
-    const cuuint32_t tile = a.slot_tokens.rows / 2;
+    using S = PromptShape<WIDTH, TILES>;
+    a.set_tile(kPromptTile, TILES);
+    const cuuint32_t tile = a.slot_tokens.rows / TILES;
     using Dim = cuuint64_t;
     CUtensorMap map_q, map_k, map_v;
     const Dim q_dims[4] = {Dim(a.width), Dim(a.group), Dim(a.queries.rows), Dim(a.kv_heads)};
@@ -434,11 +446,11 @@ cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* err
     if (!make_attention_map(&map_q, a.q, BF16, 4, q_dims, q_strides, q_box, error) || !make_attention_map(&map_k, a.k, BF16, 3, k_dims, k_strides, k_box, error) ||
         !make_attention_map(&map_v, a.v, BF16, 3, k_dims, v_strides, k_box, error))
         return cudaErrorInvalidValue;
-    auto kernel = attention_prompt_kernel<WIDTH, BF16>;
+    auto kernel = attention_prompt_kernel<WIDTH, TILES, BF16>;
     const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
     if (status != cudaSuccess) return status;
     const int slots = packed_slots(a.queries.rows, a.slot_tokens.rows, a.queries.count);
-    return launch_dependent(kernel, dim3(slots * a.kv_heads * a.head_tiles, 1, a.splits), dim3(kPromptThreads), S::kSmemBytes, stream, map_q, map_k, map_v, a);
+    return launch_dependent(kernel, dim3(slots * a.kv_heads * a.head_tiles, 1, a.splits), dim3(S::kThreads), S::kSmemBytes, stream, map_q, map_k, map_v, a);
 }
 
 }  // namespace

@@ -91,6 +91,8 @@ SHAPES = [  # queries, keys (None: the queries' own), heads, kv_heads, width
     ([300], None, 130, 1, 8),                         # 130 of them
     ([700, 513], None, 4, 1, 128),
     ([400], [1500], 6, 2, 128),
+    ([150, 40], [7000, 6500], 8, 2, 128),
+    ([600], [6200], 3, 1, 72),
     ([1], [900], 1, 1, 24),          # 3 splits of one row: the partial results' places are odd
     ([3, 1, 1], [700, 800, 900], 1, 1, 128),
 ]
@@ -157,18 +159,19 @@ def test_empty_calls():
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("queries, keys", [([90, 90, 41], [90, 90, 41]), ([2, 3], [400, 333]), ([2], [2000]), ([700, 300], [700, 300])])
-def test_what_a_query_does_not_see_does_not_reach_it(queries, keys, bad):
-    q, k, v = operands(queries, keys, 4, 2, 64, torch.bfloat16, 6)
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("queries, keys", [([90, 90, 41], [90, 90, 41]), ([2, 3], [400, 333]), ([2], [2000]), ([700, 300], [700, 300]), ([300], [6500])])
+def test_what_a_query_does_not_see_does_not_reach_it(queries, keys, bad, width):
+    q, k, v = operands(queries, keys, 4, 2, width, torch.bfloat16, 6)
     k[keys[0] - 1, 0, 5] = bad      # the first sequence's last key and value: its last query alone sees them
     v[keys[0] - 1, 1, 7] = bad
     k[keys[0] - 1, 1] = 0
     found = ops.packed_attention(q, k, v, offsets(queries), offsets(keys))
     last = queries[0] - 1
-    check(found[:last], *one_sequence(q[:last], k[:keys[0] - 1], v[:keys[0] - 1], True, 0.125))
+    check(found[:last], *one_sequence(q[:last], k[:keys[0] - 1], v[:keys[0] - 1], True, width ** -0.5))
     assert not torch.isfinite(found[last, 2:, 7]).any() and torch.isfinite(found[last, 2:, 8:]).all()
     if len(queries) > 1:
-        check_packed(found[queries[0]:], q[queries[0]:], k[keys[0]:], v[keys[0]:], queries[1:], keys[1:], True, 0.125)
+        check_packed(found[queries[0]:], q[queries[0]:], k[keys[0]:], v[keys[0]:], queries[1:], keys[1:], True, width ** -0.5)
 
 
 @pytest.mark.parametrize("bad_q, bad_k", [([0, 30, 20, 60], [0, 20, 40, 60]), ([0, 20, 40, 60], [0, 20, 40, 61]), ([-1, 20, 40, 60], [0, 20, 40, 60]),
