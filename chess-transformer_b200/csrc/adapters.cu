@@ -17,7 +17,7 @@
 
 namespace fry {
 
-constexpr int kThinRows = 64, kThinWarps = 8;  // rows of x a block takes; its warps share K
+constexpr int kThinRows = 32, kThinWarps = 8;  // rows of x a block takes; its warps share K
 
 // 16 bytes as fp16 pairs: 8 fp16 values, or 16 int8 values. int8 widens exactly: a byte with its sign bit flipped in the
 // low bits of 1024.0's fp16 pattern is 1024 + 128 + value.
@@ -41,9 +41,9 @@ FRY_DEVICE void widen_pairs(const uint4& raw, uint32_t* pairs) {
     }
 }
 
-// A block's product of up to 64 rows of x, in `groups` of 16 (rows below `low` or from `high` on count as 0), with TILES * 8
+// A block's product of up to 32 rows of x, in `groups` of 16 (rows below `low` or from `high` on count as 0), with TILES * 8
 // rows of w (those from `columns` on count as 0), K long both: the warps take runs of K in turn and leave their sums in
-// partial [kThinWarps][64][TILES * 8]. A lane's MMA fragments come from 16-byte loads: of each run of K the four lanes of a
+// partial [kThinWarps][kThinRows][TILES * 8]. A lane's MMA fragments come from 16-byte loads: of each run of K the four lanes of a
 // quad read 16 (of int8 x against fp16 w, 16 and 32) bytes each, and the MMA's K index is assigned to what a lane holds,
 // alike for x and w (a sum over K may take it in any order). Each block reads its x and w once, so the loads bound it.
 template <bool X_INT8, bool W_INT8, int TILES, int GROUPS>
@@ -130,9 +130,9 @@ FRY_DEVICE void thin_total(const float* partial, int row, int column, float (&to
         for (int e = 0; e < COUNT; ++e) total[e] = __fadd_rn(total[e], partial[(q * kThinRows + row) * TILES * 8 + column + e]);
 }
 
-// low of 64 rows of a slot and up to TILES * 8 columns of the rank.
+// low of 32 rows of a slot and up to TILES * 8 columns of the rank.
 template <bool INT8, int TILES>
-__global__ void __launch_bounds__(kThinWarps * 32, TILES <= 2 ? 2 : 1) adapter_low_kernel(const AdapterArgs p, int M, int K) {
+__global__ void __launch_bounds__(kThinWarps * 32, TILES == 1 ? 3 : TILES <= 4 ? 2 : 1) adapter_low_kernel(const AdapterArgs p, int M, int K) {
     extern __shared__ __align__(16) float partial[];
     const int lane = threadIdx.x & 31, slot = blockIdx.x, part = blockIdx.y, rank_first = blockIdx.z * TILES * 8;
     grid_dependency_start();
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThinWarps * 32, TILES <= 2 ? 2 : 1) adapter_l
     }
 }
 
-// The whole linear for up to 64 rows, 16 columns a block: there its weights are read once and bound it, and the tensor
+// The whole linear for up to 32 rows, 16 columns a block: there its weights are read once and bound it, and the tensor
 // cores' 128-row tiles would be mostly empty (16 rows against 2048 x 2048 fp16 weights: 32 such tiles of 64 columns took
 // 15.8 us). Each block's product of x and its 16 weight rows is this kernel's; an output then adds low . up of its row's
 // adapter, rank products. The weights stream in while the kernel before this one still makes low.
