@@ -89,6 +89,8 @@ std::string adapter_refusal(int kind, int M, int N, int K, int requests, int ada
     if (N <= 0 || N % 8 != 0 || K <= 0 || K % k_unit != 0)
         return "takes N a multiple of 8 and K of " + std::to_string(k_unit) + ", got N " + std::to_string(N) + ", K " + std::to_string(K);
     if (rank <= 0 || rank % 8 != 0 || rank > 128) return "takes a rank of a multiple of 8 up to 128 (pad smaller ones with zeros), got " + std::to_string(rank);
+    if (M > 0 && fry::AdapterWorkspace(kind, M, N, requests, rank).low_rows() > 0x7fffffff)
+        return "takes fewer requests: the rows of x down^T, a row tile for each, are to stay below 2^31";
     if (adapters <= 0 || static_cast<int64_t>(adapters) * N > 0x7fffff00) return "takes 1 or more adapters, their N columns together below 2^31";
     return "";
 }

@@ -84,6 +84,7 @@ struct AdapterWorkspace {
     int tile_rows;
     size_t slots, tile_slots, slot_adapter, row_slot, total;
     AdapterWorkspace(int kind, int M, int N, int requests, int rank);
+    int64_t low_rows() const { return static_cast<int64_t>(slots) * tile_rows; }
 };
 int adapter_tile_rows(int kind, int M, int N);
 cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& adapters, const void* weight, int M, int N, int K, void* workspace,

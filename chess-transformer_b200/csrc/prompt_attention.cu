@@ -449,8 +449,12 @@ cudaError_t launch_prompt(AttentionArgs a, cudaStream_t stream, std::string* err
     auto kernel = attention_prompt_kernel<WIDTH, TILES, BF16>;
     const cudaError_t status = ensure_smem(reinterpret_cast<const void*>(kernel), S::kSmemBytes);
     if (status != cudaSuccess) return status;
-    const int slots = packed_slots(a.queries.rows, a.slot_tokens.rows, a.queries.count);
-    return launch_dependent(kernel, dim3(slots * a.kv_heads * a.head_tiles, 1, a.splits), dim3(S::kThreads), S::kSmemBytes, stream, map_q, map_k, map_v, a);
+    const int64_t blocks = static_cast<int64_t>(packed_slots(a.queries.rows, a.slot_tokens.rows, a.queries.count)) * a.kv_heads * a.head_tiles;
+    if (blocks > 0x7fffffff) {
+        if (error) *error = "more row tiles of a head than a launch takes";
+        return cudaErrorInvalidValue;
+    }
+    return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks), 1, a.splits), dim3(S::kThreads), S::kSmemBytes, stream, map_q, map_k, map_v, a);
 }
 
 }  // namespace

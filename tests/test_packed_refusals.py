@@ -106,7 +106,7 @@ def adapters(lib, int8, M=4, N=16, K=32, requests=1, adapters=1, rank=8, x=16, s
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("arguments, match", [
     ({"N": 12}, "multiple of 8"), ({"N": 0}, "multiple of 8"), ({"K": 20}, "K of"), ({"rank": 4}, "rank"), ({"rank": 136}, "rank"), ({"rank": 0}, "rank"),
-    ({"adapters": 0}, "1 or more"), ({"adapters": 1 << 28}, "2\\^31"), ({"M": -1}, "rows"), ({"requests": -1}, "requests"), ({"x": 8}, "16-byte"),
+    ({"M": 1 << 23, "requests": (1 << 24) - 1, "size": 1 << 50}, "fewer requests"), ({"adapters": 0}, "1 or more"), ({"adapters": 1 << 28}, "2\\^31"), ({"M": -1}, "rows"), ({"requests": -1}, "requests"), ({"x": 8}, "16-byte"),
     ({"x": None}, "needs x"), ({"offsets": None}, "offsets"), ({"workspace": None}, "workspace"), ({"size": 100}, "workspace"),
 ])
 def test_linears_with_adapters_refuse(lib, int8, arguments, match):
