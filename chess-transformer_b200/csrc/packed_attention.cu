@@ -1,7 +1,7 @@
 // Attention over packed sequences and over a cache (packed_attention.cuh) on warp-wide tensor steps (mma.sync), for
 // sequences of few rows or few keys, and the choice between these kernels and those of prompt_attention.cu.
 //
-// Two forms. ROW_WARPS warps of 16 rows each share tiles of keys (many queries), or KEY_WARPS warps hold the same 16 rows
+// Two forms. The block's warps of 16 rows each share tiles of keys (many queries), or KEY_WARPS warps hold the same 16 rows
 // and take different keys, each with copies and a softmax of its own, joined at the end (few queries: there the loads
 // bound the kernel, and warps that wait for no other keep them in flight). Where blocks are still fewer than the SMs, the
 // keys are also split over blocks (`splits`): each writes its m, l and o to a workspace and attention_join_kernel joins
@@ -386,8 +386,15 @@ cudaError_t launch_type(const AttentionArgs& a, const AttentionPlan& plan, cudaS
 AttentionPlan attention_plan(const AttentionShape& s) {
     AttentionPlan plan;
     const int64_t sequences = s.sequences > 0 ? s.sequences : 1;
-    const int64_t mean_rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / sequences, mean_keys = s.cached ? s.capacity : s.key_rows / sequences;
-    const bool few = s.cached || mean_rows <= 16, prompt = !few && mean_rows >= 128 && mean_keys >= 128;
+    const int64_t all_rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / sequences, mean_rows = all_rows > 0 ? all_rows : 1;
+    const int64_t mean_keys = s.cached ? s.capacity : s.key_rows / sequences;
+    // Few rows against enough keys: the key warps (64 x 2 tokens of 8 grouped heads, 2000 keys, 48 us against the row
+    // warps' 171; but 256 x 8 tokens against 8 keys 34 against 21). More rows: the prompt kernel, where its tiles of 128
+    // rows and keys are filled well enough (64 x 64 tokens, 512 keys, 41 us against 59; x 128, 128 keys, 28 against 43; x 4
+    // of 8 grouped heads, 2000 keys, 56 against 84 of the key warps; but 64 x 32 tokens, 256 keys, 28 against 22, and 128 x
+    // 70 of 2 grouped heads, 70 keys, 80 against 52).
+    const bool few = s.cached || (mean_rows <= 16 && mean_keys >= 128);
+    const bool prompt = !few && mean_rows > 16 && mean_keys >= 128 && mean_rows * mean_keys >= 128 * 128;
     plan.form = few ? AttentionForm::kFew : prompt ? AttentionForm::kPrompt : AttentionForm::kRows;
     // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
     const int64_t group = s.heads / s.kv_heads;

@@ -48,6 +48,15 @@ def test_workspaces_are_sized_by_the_shape(lib):
     assert lib.fry_packed_attention_workspace_bytes(1, 32768, 1, 32, 5, 128) == 0  # a refused shape
 
 
+def test_every_shape_has_a_plan(lib):
+    """Fewer rows than sequences, none, or one of many keys: the choice of kernel and splits divides by none of them."""
+    for rows in (0, 1, 3, 200, 100000):
+        for keys in (0, 1, 127, 128, 5000, 1 << 20):
+            for sequences in (0, 1, 7, 5000):
+                for heads, kv_heads in ((1, 1), (24, 12), (130, 1)):
+                    assert lib.fry_packed_attention_workspace_bytes(rows, keys, sequences, heads, kv_heads, 64) >= 0
+
+
 def test_cpu_tensors_are_refused():
     q = torch.zeros(3, 4, 64, dtype=torch.float16)
     at = torch.tensor([0, 3], dtype=torch.int32)
