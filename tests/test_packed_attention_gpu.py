@@ -93,6 +93,10 @@ SHAPES = [  # queries, keys (None: the queries' own), heads, kv_heads, width
     ([400], [1500], 6, 2, 128),
     ([150, 40], [7000, 6500], 8, 2, 128),
     ([600], [6200], 3, 1, 72),
+    ([20], [700], 1, 1, 64),
+    ([300, 310] * 10, None, 16, 8, 128),
+    ([260] * 6, [6200] * 6, 32, 8, 128),
+    ([1, 2, 0, 1] * 30, [200, 130, 150, 333] * 30, 8, 4, 64),
     ([1], [900], 1, 1, 24),          # 3 splits of one row: the partial results' places are odd
     ([3, 1, 1], [700, 800, 900], 1, 1, 128),
 ]
