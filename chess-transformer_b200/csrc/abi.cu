@@ -57,6 +57,7 @@ std::string attention_refusal(const fry::AttentionShape& s) {
     if (s.kv_heads <= 0 || s.heads <= 0 || s.heads > 1024 || s.heads % s.kv_heads != 0)
         return "takes 1 to 1024 query heads, a multiple of the key/value heads, got " + std::to_string(s.heads) + " and " + std::to_string(s.kv_heads);
     if (s.width <= 0 || s.width > 128 || s.width % 8 != 0) return "takes heads a multiple of 8 up to 128 wide, got " + std::to_string(s.width);
+    if (s.key_rows > (1 << 30)) return "takes up to 2^30 key rows";
     if (s.q_rows > fry::kMaxPackedRows || s.sequences > fry::kMaxPackedRows) return "takes up to 2^24 - 1 query rows and sequences";
     return "";
 }
@@ -64,7 +65,7 @@ std::string attention_refusal(const fry::AttentionShape& s) {
 int run_attention(const char* name, const fry::AttentionShape& shape, const fry::AttentionTensors& x, float scale, void* workspace,
                   size_t workspace_bytes, void* stream) {
     std::string refusal = attention_refusal(shape);
-    if (refusal.empty() && !(scale > 0.0f && scale <= 3.0e38f)) refusal = "takes a positive, finite scale";
+    if (refusal.empty() && !(scale > 0.0f && scale <= 2.0e38f)) refusal = "takes a positive scale up to 2e38";
     if (refusal.empty()) {
         for (int64_t stride : {x.q_row, x.q_head, x.k_row, x.k_head, x.v_row, x.v_head, x.k_sequence, x.v_sequence})
             if (stride < 0 || stride % 8 != 0) refusal = "takes strides of a multiple of 8 elements";

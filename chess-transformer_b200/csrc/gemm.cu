@@ -29,6 +29,8 @@
 // the even CTA's stage barrier; the even CTA's MMA warp issues the pair's MMAs and commits to the stage and accumulator
 // barriers of both CTAs; each CTA's epilogue reads its own TMEM (its 128 rows) and returns the accumulator to the even
 // CTA's barrier. A tile is then 256 rows, and each CTA moves half the B bytes.
+// Adapters (adapters.cu): a tile's K steps are followed by one a request of the tile that has an adapter, low's rows against
+// up's, into the same accumulator (kind::f16) or an fp32 one beside the int32 sums (kind::i8), whose columns halve the tile.
 // No TMA load multicasts.
 #include <mutex>
 #include <string>

@@ -79,7 +79,8 @@ int fry_int8_linear_normed(const uint16_t* x, const uint16_t* gain, float eps, c
  * request), and
  *   out[m] = fp16((fma(acc * x_scale, weight_scale, bias) + (x_scale x[m] down[a]^T) up[a]^T) + residual[m])
  * down fp16 [adapters, rank, K], up fp16 [adapters, N, rank] (a scale of the adapter is the caller's, in either); the
- * adapters' sums fp32, x down^T rounded to fp16 between the two products. bias and residual fp16, either NULL: none. An
+ * adapters' sums fp32, x down^T rounded to fp16 between the two products (beyond 65504 it is infinite); up to 32 rows acc
+ * is summed in fp32 too. bias and residual fp16, either NULL: none. An
  * adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids out of range are recorded in the device
  * status (code 7, where = the request): ids count as -1, rows of such offsets hold unspecified values. rank a multiple of 8
  * up to 128, N of 8, K of 16, adapters * N below 2^31, M and requests below 2^24; out overlaps no input but residual;
@@ -126,7 +127,7 @@ int fry_attention_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
  * outside their tensor or descending are read as the nearest row and recorded (code 7, where = the sequence); what the
  * rows then hold is unspecified. out [q_rows, heads, head_dim] is dense and overlaps no input; strides are in elements,
  * multiples of 8, the last axis dense; q, k, v and out 16-byte aligned. head_dim a multiple of 8 up to 128, heads a multiple of
- * kv_heads up to 1024, rows and sequences below 2^24, scale positive. workspace: 16-byte aligned, of fry_packed_attention_workspace_bytes (0 where the
+ * kv_heads up to 1024, query rows and sequences below 2^24, key rows up to 2^30, scale positive, up to 2e38. workspace: 16-byte aligned, of fry_packed_attention_workspace_bytes (0 where the
  * keys are not split over blocks). Calls whose work overlaps on the GPU need workspaces of their own. The reference has
  * no attention of this form: its template attention (model/fused_blocks.py:54-97) sees 70 tokens, all of them. */
 size_t fry_packed_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim);

@@ -199,6 +199,24 @@ def test_recorded_into_two_graphs_on_a_side_stream(int8):
             assert torch.equal(out, case.run())
 
 
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU have workspaces of their own."""
+    cases = [Case(int8, [70] * 40 + [900], [i % 4 - 1 for i in range(41)], 3, 16, 768, 1440, seed=40 + i) for i, int8 in enumerate((False, True))]
+    q = torch.randn(3, 8, 64, device="cuda").half()
+    cache = torch.randn(3, 4000, 2, 64, device="cuda").half()
+    lengths = int32([4000, 17, 2500])
+    expected = [case.run() for case in cases] + [ops.cached_attention(q, cache, cache, lengths)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    found = [[], []]
+    for _ in range(20):
+        for stream, outs in zip(streams, found):
+            with torch.cuda.stream(stream):
+                outs.append([case.run() for case in cases] + [ops.cached_attention(q, cache, cache, lengths)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, right) for outs in found for call in outs for out, right in zip(call, expected))
+
+
 def test_the_same_call_gives_the_same_bits():
     for int8 in (False, True):
         case = Case(int8, [70] * 30, [i % 5 - 1 for i in range(30)], 4, 16, 768, 1440, seed=28)

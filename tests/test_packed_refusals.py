@@ -28,7 +28,8 @@ def packed(lib, q_rows=4, k_rows=4, sequences=1, heads=4, kv_heads=2, width=64, 
     ({"width": 12}, "multiple of 8"), ({"width": 136}, "up to 128"), ({"width": 0}, "up to 128"), ({"q_rows": -1}, ">= 0"), ({"sequences": -1}, ">= 0"),
     ({"scale": 0.0}, "positive"), ({"scale": -1.0}, "positive"), ({"scale": float("nan")}, "positive"), ({"scale": float("inf")}, "positive"),
     ({"strides": (256, 64, 128, 60, 128, 64)}, "strides"), ({"strides": (-256, 64, 128, 64, 128, 64)}, "strides"), ({"q": 24}, "16-byte"),
-    ({"offsets": None}, "offsets"), ({"out": None}, "needs q"), ({"sequences": 1 << 27}, "2\\^24"),
+    ({"offsets": None}, "offsets"), ({"out": None}, "needs q"), ({"sequences": 1 << 27}, "2\\^24"), ({"k_rows": (1 << 30) + 1}, "2\\^30"),
+    ({"scale": 3e38}, "2e38"),
     ({"q_rows": 2, "k_rows": 100000, "workspace": 16, "size": 8}, "workspace"), ({"q_rows": 2, "k_rows": 100000}, "workspace"),
 ])
 def test_packed_attention_refuses(lib, arguments, match):
