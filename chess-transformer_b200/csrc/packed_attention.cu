@@ -26,7 +26,7 @@ FRY_DEVICE void cp_async16_or_zero(uint32_t shared, const void* global, bool rea
 // keys; more, they have the same rows and KEYS keys each of a stage.
 //
 // What bounds them: the key warps HBM (64 full caches of 8192 keys, 8 heads of 128: 6.7 TB/s; of 2048, 12 heads of 64: 5.0 TB/s,
-// 4.5 with uneven lengths). The row warps the instructions: of 62 us for 256 x 70 tokens, 24 heads of 32, 20 go to the
+// 4.5 with uneven lengths). The row warps the instructions: at 64 keys a stage, of 62 us for 256 x 70 tokens, 24 heads of 32, 20 go to the
 // search, the queries and the outputs, 13 to the copies and 29 to products and softmax.
 constexpr int kMaxRowWarps = 8;
 template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES>
@@ -366,9 +366,11 @@ cudaError_t launch_rows(AttentionArgs a, int row_warps, cudaStream_t stream) {
     return launch_dependent(kernel, dim3(slots, a.kv_heads * a.head_tiles, a.splits), dim3(warps * 32), smem, stream, a);
 }
 
+// Width 32, whose blocks have 64 registers a thread: 48 keys a stage spill less than 64 and waste less of a last stage (256 x
+// 70 tokens, 61.4 -> 58.2 us; 200 x 96, 64.9 -> 58.6; 700 x 24, 48.0 -> 44.5; but 256 x 64, 45.7 -> 46.5; 80: 67.9, 96: 73.0).
 template <int WIDTH, bool BF16>
 cudaError_t launch_width(const AttentionArgs& a, const AttentionPlan& plan, cudaStream_t stream) {
-    return plan.form == AttentionForm::kFew ? launch_rows<WIDTH, 4, 16, 3, BF16>(a, 1, stream) : launch_rows<WIDTH, 1, 64, 2, BF16>(a, plan.row_warps, stream);
+    return plan.form == AttentionForm::kFew ? launch_rows<WIDTH, 4, 16, 3, BF16>(a, 1, stream) : launch_rows<WIDTH, 1, WIDTH == 32 ? 48 : 64, 2, BF16>(a, plan.row_warps, stream);
 }
 
 template <bool BF16>

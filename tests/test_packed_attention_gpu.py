@@ -99,6 +99,8 @@ SHAPES = [  # queries, keys (None: the queries' own), heads, kv_heads, width
     ([1, 2, 0, 1] * 30, [200, 130, 150, 333] * 30, 8, 4, 64),
     ([1], [900], 1, 1, 24),          # 3 splits of one row: the partial results' places are odd
     ([3, 1, 1], [700, 800, 900], 1, 1, 128),
+    ([47, 48, 49, 20, 30, 40, 33], [47, 48, 49, 95, 96, 97, 113], 6, 2, 32),  # keys about a stage's end
+    ([20, 17, 35], [15, 47, 145], 3, 3, 24),
 ]
 
 
