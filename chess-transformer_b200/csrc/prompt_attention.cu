@@ -1,5 +1,5 @@
-// Attention over packed sequences on the fifth-generation tensor cores, for sequences of many rows (packed_attention.cu has
-// the operator's definition, the other kernels and the choice between them).
+// Attention over packed sequences on the fifth-generation tensor cores, for sequences of many rows (packed_attention.cuh has
+// the operator's definition, packed_attention.cu the other kernels and the choice between them).
 //
 // A block takes TILES tiles of 128 rows (a row is a token and one of the query heads that share its keys) against keys in
 // tiles of 128, each of the products a tcgen05.mma of M = 128: scores S = Q K^T into TMEM, and O += P V with P read from
