@@ -145,7 +145,7 @@ def _(q, k, v, heads):
 
 
 # The packed operators below check a call in one expression and go on; where it does not hold, a second function finds out
-# what to say. A small call is bound by this host code (5.5 us of 13 are the library's, the rest torch's and Python's).
+# what to say: a small call is bound by host code, of which torch's dispatcher is the larger part.
 
 def _call(function, index: int, *arguments) -> None:
     """A library call on device `index` and its current stream, whatever device is current."""
@@ -154,14 +154,6 @@ def _call(function, index: int, *arguments) -> None:
     else:
         with torch.cuda.device(index):
             function(*arguments, torch._C._cuda_getCurrentRawStream(index))
-
-
-def _direct(*tensors: torch.Tensor | None) -> bool:
-    """Whether a call may skip torch's dispatcher (about 12 us of a small call): not under torch.compile, which must see
-    the op, nor on fake tensors or where autograd would record it."""
-    if torch.compiler.is_compiling() or type(tensors[0]) is not torch.Tensor:
-        return False
-    return not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors)
 
 
 def _index32(name: str, tensor: torch.Tensor, what: str, count: int, device: torch.device) -> None:
@@ -203,7 +195,16 @@ def _workspace_bytes(function: str, *shape: int) -> int:
     return getattr(library(), function)(*shape)
 
 
-def _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale):
+@torch.library.custom_op("fry::packed_attention", mutates_args=())
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor, causal: bool = True,
+                     scale: float | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over sequences packed one behind the other (the op fry::packed_attention): q [rows, heads,
+    width], k and v [key rows, kv_heads, width], fp16 or bf16, query head h on key/value head h // (heads // kv_heads);
+    sequence s has the rows q_offsets[s] to q_offsets[s + 1] and the keys k_offsets[s] to k_offsets[s + 1] (int32, on the
+    device). Causal, its queries are its last tokens: query i of nq sees keys j <= i + nk - nq. Rows that see no key, and
+    rows of no sequence, are 0. width a multiple of 8 up to 128; scale defaults to 1 / sqrt(width). No backward pass.
+    Strided views (of a projection's rows, say) are read in place where their last axis is dense and their other strides
+    are multiples of 8."""
     q_shape, k_shape, dtype, index = q.shape, k.shape, q.dtype, q.get_device()
     shaped = (len(q_shape) == 3 and len(k_shape) == 3 and v.shape == k_shape and q_shape[2] == k_shape[2] and k_shape[1] > 0
               and q_shape[1] % k_shape[1] == 0)
@@ -227,31 +228,16 @@ def _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale):
     return out
 
 
-@torch.library.custom_op("fry::packed_attention", mutates_args=())
-def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor, causal: bool,
-                         scale: float | None) -> torch.Tensor:
-    return _packed_attention(q, k, v, q_offsets, k_offsets, causal, scale)
-
-
-@_packed_attention_op.register_fake
-def _(q, k, v, q_offsets, k_offsets, causal, scale):
+@packed_attention.register_fake
+def _(q, k, v, q_offsets, k_offsets, causal=True, scale=None):
     return q.new_empty(q.shape)
 
 
-def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor, causal: bool = True,
-                     scale: float | None = None) -> torch.Tensor:
-    """softmax(scale q k^T) v over sequences packed one behind the other (the op fry::packed_attention): q [rows, heads,
-    width], k and v [key rows, kv_heads, width], fp16 or bf16, query head h on key/value head h // (heads // kv_heads);
-    sequence s has the rows q_offsets[s] to q_offsets[s + 1] and the keys k_offsets[s] to k_offsets[s + 1] (int32, on the
-    device). Causal, its queries are its last tokens: query i of nq sees keys j <= i + nk - nq. Rows that see no key, and
-    rows of no sequence, are 0. width a multiple of 8 up to 128; scale defaults to 1 / sqrt(width). No backward pass.
-    Strided views (of a projection's rows, say) are read in place where their last axis is dense and their other strides
-    are multiples of 8."""
-    run = _packed_attention if _direct(q, k, v) else torch.ops.fry.packed_attention
-    return run(q, k, v, q_offsets, k_offsets, causal, scale)
-
-
-def _cached_attention(q, k, v, lengths, scale):
+@torch.library.custom_op("fry::cached_attention", mutates_args=())
+def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float | None = None) -> torch.Tensor:
+    """packed_attention for one query token a sequence over a cache (the op fry::cached_attention): q [sequences, heads,
+    width], k and v [sequences, capacity, kv_heads, width] by any strides, of which sequence s has its first lengths[s] keys
+    (int32, on the device). What lies behind a length is not read; a length of 0 answers 0."""
     q_shape, k_shape, dtype, index = q.shape, k.shape, q.dtype, q.get_device()
     shaped = (len(q_shape) == 3 and len(k_shape) == 4 and v.shape == k_shape and k_shape[0] == q_shape[0] and q_shape[2] == k_shape[3]
               and k_shape[2] > 0 and q_shape[1] % k_shape[2] == 0)
@@ -272,22 +258,9 @@ def _cached_attention(q, k, v, lengths, scale):
     return out
 
 
-@torch.library.custom_op("fry::cached_attention", mutates_args=())
-def _cached_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float | None) -> torch.Tensor:
-    return _cached_attention(q, k, v, lengths, scale)
-
-
-@_cached_attention_op.register_fake
-def _(q, k, v, lengths, scale):
+@cached_attention.register_fake
+def _(q, k, v, lengths, scale=None):
     return q.new_empty(q.shape)
-
-
-def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float | None = None) -> torch.Tensor:
-    """packed_attention for one query token a sequence over a cache (the op fry::cached_attention): q [sequences, heads,
-    width], k and v [sequences, capacity, kv_heads, width] by any strides, of which sequence s has its first lengths[s] keys
-    (int32, on the device). What lies behind a length is not read; a length of 0 answers 0."""
-    run = _cached_attention if _direct(q, k, v) else torch.ops.fry.cached_attention
-    return run(q, k, v, lengths, scale)
 
 
 def _aligned(tensor: torch.Tensor) -> torch.Tensor:
@@ -337,7 +310,14 @@ def _adapter_operands(name: str, x, weight, bias, residual, down, up, offsets, i
     return index, (x.numel() // K if K else 0, N, K, ids.shape[0], down_shape[0], down_shape[1]), operands
 
 
-def _adapter_linear(x, weight, bias, residual, down, up, offsets, ids):
+@torch.library.custom_op("fry::adapter_linear", mutates_args=())
+def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None, down: torch.Tensor,
+                   up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """A linear with a low-rank adapter for each request's rows (the op fry::adapter_linear), fp16:
+    x W^T + bias + residual, plus (x down[a]^T) up[a]^T for the rows offsets[s] to offsets[s + 1] of request s, a = ids[s].
+    x [..., K], weight [N, K] as nn.Linear holds it, down [adapters, rank, K], up [adapters, N, rank]; offsets [requests + 1]
+    and ids [requests] int32 on the device; rows of no request and those of ids -1 have no adapter. rank a multiple of 8 up
+    to 128 (pad smaller ones with zeros), N and K multiples of 8. No backward pass."""
     index, shapes, operands = _adapter_operands("adapter_linear", x, weight, bias, residual, down, up, offsets, ids, torch.float16)
     M, N, _, requests, _, rank = shapes
     out = x.new_empty(*x.shape[:-1], N)
@@ -347,29 +327,17 @@ def _adapter_linear(x, weight, bias, residual, down, up, offsets, ids):
     return out
 
 
-@torch.library.custom_op("fry::adapter_linear", mutates_args=())
-def _adapter_linear_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None, down: torch.Tensor,
-                       up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
-    return _adapter_linear(x, weight, bias, residual, down, up, offsets, ids)
-
-
-@_adapter_linear_op.register_fake
+@adapter_linear.register_fake
 def _(x, weight, bias, residual, down, up, offsets, ids):
     return x.new_empty(*x.shape[:-1], weight.shape[0])
 
 
-def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None, down: torch.Tensor,
-                   up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
-    """A linear with a low-rank adapter for each request's rows (the op fry::adapter_linear), fp16:
-    x W^T + bias + residual, plus (x down[a]^T) up[a]^T for the rows offsets[s] to offsets[s + 1] of request s, a = ids[s].
-    x [..., K], weight [N, K] as nn.Linear holds it, down [adapters, rank, K], up [adapters, N, rank]; offsets [requests + 1]
-    and ids [requests] int32 on the device; rows of no request and those of ids -1 have no adapter. rank a multiple of 8 up
-    to 128 (pad smaller ones with zeros), N and K multiples of 8. No backward pass."""
-    run = _adapter_linear if _direct(x, weight, bias, residual, down, up) else torch.ops.fry.adapter_linear
-    return run(x, weight, bias, residual, down, up, offsets, ids)
-
-
-def _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids):
+@torch.library.custom_op("fry::int8_adapter_linear", mutates_args=())
+def int8_adapter_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None,
+                        residual: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    """adapter_linear beside the int8 linear (the op fry::int8_adapter_linear): x int8 [..., K] with x_scale fp32 a row,
+    weight int8 [N, K] with weight_scale fp32 a row, as int8_linear takes them; the adapters fp16, on the rows that x and
+    x_scale stand for. K a multiple of 16."""
     name = "int8_adapter_linear"
     index, shapes, (x, weight, *others) = _adapter_operands(name, x, weight, bias, residual, down, up, offsets, ids, torch.int8)
     M, N, _, requests, _, rank = shapes
@@ -386,25 +354,9 @@ def _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down,
     return out
 
 
-@torch.library.custom_op("fry::int8_adapter_linear", mutates_args=())
-def _int8_adapter_linear_op(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None,
-                            residual: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor,
-                            ids: torch.Tensor) -> torch.Tensor:
-    return _int8_adapter_linear(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids)
-
-
-@_int8_adapter_linear_op.register_fake
+@int8_adapter_linear.register_fake
 def _(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids):
     return x.new_empty(*x.shape[:-1], weight.shape[0], dtype=torch.float16)
-
-
-def int8_adapter_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None,
-                        residual: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor, offsets: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
-    """adapter_linear beside the int8 linear (the op fry::int8_adapter_linear): x int8 [..., K] with x_scale fp32 a row,
-    weight int8 [N, K] with weight_scale fp32 a row, as int8_linear takes them; the adapters fp16, on the rows that x and
-    x_scale stand for. K a multiple of 16."""
-    run = _int8_adapter_linear if _direct(x, x_scale, weight_scale, bias, residual, down, up) else torch.ops.fry.int8_adapter_linear
-    return run(x, x_scale, weight, weight_scale, bias, residual, down, up, offsets, ids)
 
 
 @torch.library.custom_op("fry::norm_quant", mutates_args=())
