@@ -243,10 +243,6 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
 #pragma unroll
             for (int i = 0; i < WIDTH / 32; ++i) finite = finite && isfinite(joined[i]);
             const int token = token_of(r), head = head_of(r);
-            if (isfinite(total) && !__all_sync(0xffffffffu, finite)) {
-                recompute_row<BF16>(a, b, token, head, low, min(high, b.limit(token, a.causal)), split, lane);
-                continue;
-            }
             const AttentionOut to = attention_out(a, split, b.row + token, head);
             const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
@@ -257,6 +253,9 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
                 else to.out[c] = static_cast<uint16_t>(pack16<BF16>(joined[i] * inverse, 0.0f) & 0xffff);
             }
             if (a.splits > 1 && lane == 0) to.part_sums[0] = top, to.part_sums[1] = total;
+            auto row_at = [&](int, int& its_token, int& its_head) { its_token = token, its_head = head; };
+            if (isfinite(total) && !__all_sync(0xffffffffu, finite))
+                repair_rows<BF16>(a, b, 1, total == 0.0f ? 1 : 0, row_at, low, high, high, split, lane);
         }
     } else {
         uint8_t* staged = smem + warp * 16 * WIDTH * 2;
@@ -295,14 +294,17 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
                         *reinterpret_cast<const uint4*>(staged + tile_unit<WIDTH>(r, unit));
             }
         }
-        __syncwarp();
         if (__all_sync(0xffffffffu, finite[0] && finite[1])) return;
-        for (int i = 0; i < 16; ++i) {  // rows whose output is not finite though their sum is
-            const uint32_t votes = __ballot_sync(0xffffffffu, !finite[i / 8]);
-            if (((votes >> (i % 8 * 4)) & 15u) == 0) continue;
-            const int r = row_warp * 16 + i, token = token_of(r);
-            recompute_row<BF16>(a, b, token, head_of(r), low, min(high, b.limit(token, a.causal)), split, lane);
-        }
+        // rows whose output is not finite though their sum is, and those without a sum, from the votes of their quads
+        auto rows_of = [&](bool first, bool second) {
+            const uint32_t low8 = __ballot_sync(0xffffffffu, first), high8 = __ballot_sync(0xffffffffu, second);
+            uint32_t rows = 0;
+            for (int i = 0; i < 16; ++i) rows |= (((i < 8 ? low8 : high8) >> (i % 8 * 4)) & 15u) != 0 ? 1u << i : 0u;
+            return rows;
+        };
+        const uint32_t again = rows_of(!finite[0], !finite[1]), empty = rows_of(l[0] == 0.0f, l[1] == 0.0f);
+        auto row_at = [&](int i, int& token, int& head) { token = token_of(row_warp * 16 + i), head = head_of(row_warp * 16 + i); };
+        repair_rows<BF16>(a, b, again, empty, row_at, low, high, high, split, lane);
     }
 }
 
