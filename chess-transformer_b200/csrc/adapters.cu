@@ -240,6 +240,98 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
     }
 }
 
+// x . y over `count` fp16 values, a multiple of 8, both on 16 bytes.
+FRY_DEVICE float dot16(const uint16_t* x, const uint16_t* y, int count) {
+    float sum = 0.0f;
+    for (int k = 0; k < count; k += 8) {
+        float a[8], b[8];
+        unpack8(*reinterpret_cast<const uint4*>(x + k), a);
+        unpack8(*reinterpret_cast<const uint4*>(y + k), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __fmaf_rn(a[e], b[e], sum);
+    }
+    return sum;
+}
+
+// A sum that is not finite stands where no other request of the tile has an adapter that is not finite in its column: it is
+// the row's own then. The others are the row's x . w (kEpiAdapterF16; a warp's 32 x 16 of them on mma.sync, its fragments as in
+// thin_product_of) plus low . up of its own request. 3744 rows through 2048 x 2048, rank 32, 50 us a call: 86 us with an x
+// that is not finite in every row, 1.08 ms with a quarter of the requests on a NaN adapter; summed again in scalars, 79 ms.
+template <int EPI>
+__device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, int column, uint32_t* sums) {
+    const int lane = threadIdx.x & 31, first_row = m - lane, tile_rows = p.adapters.tile_rows, tile = first_row / tile_rows, rank = p.adapters.rank;
+    uint32_t bad = 0;  // of this lane's row, by column
+    for (int e = 0; e < 16; ++e)
+        if (m < p.M && column + e < p.N && !isfinite(__uint_as_float(sums[e]))) bad |= 1u << e;
+    const int2 slots = adapter_slots(p, tile);
+    uint32_t reached = 0;
+    int own_slot = -1, own_adapter = 0;
+    for (int slot = slots.x; slot < slots.y; ++slot) {
+        const int adapter = p.adapters.slot_adapter[slot], request = slot - tile - 1;
+        if (adapter < 0 || adapter >= p.adapters.adapters || request < 0 || request >= p.adapters.requests) continue;
+        const bool mine = m >= p.adapters.offsets[request] && m < p.adapters.offsets[request + 1];
+        if (mine) own_slot = slot, own_adapter = adapter;
+        // lane i looks at half of the rank in column i % 16
+        bool found = false;
+        if (column + lane % 16 < p.N) {
+            const uint16_t* up = p.adapters.up + (static_cast<size_t>(adapter) * p.N + column + lane % 16) * rank;
+            for (int j = lane / 16 * 8; j < rank; j += 16) {
+                const uint4 words = __ldg(reinterpret_cast<const uint4*>(up + j));
+                for (uint32_t w : {words.x, words.y, words.z, words.w}) found = found || (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+            }
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, found);
+        if (!mine) reached |= (votes | votes >> 16) & 0xffffu;
+    }
+    const uint32_t again = bad & reached;
+    if (!__any_sync(0xffffffffu, again != 0)) return;
+
+    float total[2][2][4] = {};  // rows in two 16s, columns in two 8s
+    if constexpr (EPI == kEpiAdapterF16) {
+        const int g = lane >> 2, t = lane & 3;
+        const uint16_t* x = static_cast<const uint16_t*>(p.adapters.x);
+#pragma unroll 2
+        for (int k = t * 8; k - t * 8 < p.K; k += 32) {
+            uint4 a[2][2], b[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                b[n] = k < p.K && column + n * 8 + g < p.N ? __ldg(reinterpret_cast<const uint4*>(p.weight + static_cast<size_t>(column + n * 8 + g) * p.K + k))
+                                                           : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int row = first_row + i * 16 + half * 8 + g;
+                    a[i][half] = k < p.K && row < p.M ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(row) * p.K + k) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma_f16(total[i][n], a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b[n].x, b[n].y);
+                    mma_f16(total[i][n], a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b[n].z, b[n].w);
+                }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        // element (lane, e) is in lane (lane % 8) * 4 + e % 8 / 2, of its rows' 16 and 8
+        float sum = 0.0f;
+        if constexpr (EPI == kEpiAdapterF16) {
+#pragma unroll
+            for (int quarter = 0; quarter < 4; ++quarter) {
+                const float found = __shfl_sync(0xffffffffu, total[quarter / 2][e / 8][quarter % 2 * 2 + e % 2], lane % 8 * 4 + e % 8 / 2);
+                if (lane / 8 == quarter) sum = found;
+            }
+        }
+        if (!((again >> e) & 1)) continue;
+        if (own_slot >= 0)
+            sum += dot16(p.adapters.low + (static_cast<size_t>(own_slot) * tile_rows + m % tile_rows) * rank,
+                         p.adapters.up + (static_cast<size_t>(own_adapter) * p.N + column + e) * rank, rank);
+        sums[e] = __float_as_uint(sum);
+    }
+}
+
 namespace {
 
 constexpr int kThinMost = 32;  // rows up to which the thin kernel takes the linear

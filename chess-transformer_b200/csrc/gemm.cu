@@ -353,42 +353,26 @@ FRY_DEVICE int2 adapter_slots(const AdapterGemmArgs& p, int row_tile) {
     return slots.x >= 0 && slots.y <= p.slots ? slots : make_int2(0, 0);
 }
 
-// The sums of element (m, n) from its own request's adapter alone (kEpiAdapterF16: with x . weight). A tile's adapter steps
-// multiply the rows of other requests by zeros, so an adapter that is not finite makes them NaN: elements that are not
-// finite are summed again this way, whatever made them so. Slow, and seldom run.
+// A tile's adapter steps multiply the rows of other requests by zeros, so an adapter that is not finite makes them NaN. Looks
+// at a warp's 32 rows of 16 sums, some not finite, and takes those again that another request's adapter has reached
+// (adapters.cu). m: this lane's row, of 32 in order.
 template <int EPI>
-__device__ __noinline__ float adapter_sums(const AdapterGemmArgs& p, int m, int n) {
-    float sum = 0.0f;
-    if constexpr (EPI == kEpiAdapterF16) {
-        const uint16_t* x = static_cast<const uint16_t*>(p.adapters.x) + static_cast<size_t>(m) * p.K;
-        const uint16_t* w = p.weight + static_cast<size_t>(n) * p.K;
-        for (int k = 0; k < p.K; ++k) sum = __fmaf_rn(h2f_bits(x[k]), h2f_bits(w[k]), sum);
-    }
-    const int tile = m / p.adapters.tile_rows, rank = p.adapters.rank;
-    const int2 slots = adapter_slots(p, tile);
-    for (int slot = slots.x; slot < slots.y; ++slot) {
-        const int adapter = p.adapters.slot_adapter[slot], request = slot - tile - 1;
-        if (adapter < 0 || adapter >= p.adapters.adapters || request < 0 || request >= p.adapters.requests) continue;
-        if (m < p.adapters.offsets[request] || m >= p.adapters.offsets[request + 1]) continue;
-        const uint16_t* low = p.adapters.low + (static_cast<size_t>(slot) * p.adapters.tile_rows + m % p.adapters.tile_rows) * rank;
-        const uint16_t* up = p.adapters.up + (static_cast<size_t>(adapter) * p.N + n) * rank;
-        for (int j = 0; j < rank; ++j) sum = __fmaf_rn(h2f_bits(low[j]), h2f_bits(up[j]), sum);
-    }
-    return sum;
-}
-// A row's 16 sums from `column` on, those that are not finite summed again (rows and columns of the output alone).
+__device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, int column, uint32_t* sums);
+
+// A row's 16 sums from `column` on, with none of other requests' adapters in them. Every lane of the warp calls it.
 template <int EPI>
-FRY_DEVICE void finite_sums(const AdapterGemmArgs& p, size_t row, int column, uint32_t (&sums)[16]) {
+FRY_DEVICE void own_sums(const AdapterGemmArgs& p, size_t row, int column, uint32_t (&sums)[16]) {
     uint64_t zero2 = pair2(0.0f, 0.0f);  // 0 * sum is 0 where the sum is finite, else NaN
 #pragma unroll
     for (int e = 0; e < 16; e += 2) zero2 = fma2(pair2(__uint_as_float(sums[e]), __uint_as_float(sums[e + 1])), pair2(0.0f, 0.0f), zero2);
     const float2 zero = lanes(zero2);
-    if (zero.x + zero.y == 0.0f) return;
-    const int m = static_cast<int>((row - column) / p.N);
-    if (m >= p.M) return;
+    if (!__any_sync(0xffffffffu, zero.x + zero.y != 0.0f)) return;
+    uint32_t copy[16];  // (so that the sums stay in registers where all are finite)
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-        if (column + e < p.N && !isfinite(__uint_as_float(sums[e]))) sums[e] = __float_as_uint(adapter_sums<EPI>(p, m, column + e));
+    for (int e = 0; e < 16; ++e) copy[e] = sums[e];
+    take_sums_again<EPI>(p, static_cast<int>((row - column) / p.N), column, copy);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[e] = copy[e];
 }
 
 // Applies the epilogue to one row's 16 consecutive columns. acc (and up, gated) hold the raw TMEM words, xs the row's
@@ -419,8 +403,8 @@ FRY_DEVICE void epilogue16(const ArgsOf<EPI>& p, float xs, float rs, float is, u
             }
         return;
     } else {
-        if constexpr (EPI == kEpiAdapterF16) finite_sums<EPI>(p, row, column, acc);
-        if constexpr (EPI == kEpiAdapterInt8) finite_sums<EPI>(p, row, column, up);
+        if constexpr (EPI == kEpiAdapterF16) own_sums<EPI>(p, row, column, acc);
+        if constexpr (EPI == kEpiAdapterInt8) own_sums<EPI>(p, row, column, up);
         constexpr bool kResidual = EPI == kEpiResidual || mixes(EPI) || optional_residual(EPI);
         uint4 residual_words[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, original_words[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if constexpr (kResidual) {
@@ -995,6 +979,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 const int slot = j % S::kSlots;
                 if (has_rows && !mbar_wait(&rows_full[slot], (j / S::kSlots) & 1, 14)) alive = false;
                 uint8_t* staged_sub = io + slot * S::kSlotBytes;
+                if constexpr (adapts(EPI)) alive = __all_sync(0xffffffffu, alive);  // own_sums() votes in whole warps
                 if (alive) {
                     tc_fence_after();
 #pragma unroll
