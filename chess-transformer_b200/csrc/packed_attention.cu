@@ -32,8 +32,9 @@ constexpr int kMaxRowWarps = 8;
 template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES>
 struct RowsShape {
     static constexpr int kMaxThreads = (KEY_WARPS > 1 ? KEY_WARPS : kMaxRowWarps) * 32;
-    // blocks an SM: 8 warps of a narrow head in 64 registers a thread, 4 times over, hide the loads' latency
-    static constexpr int kBlocks = KEY_WARPS > 1 ? 1 : WIDTH == 32 ? 4 : WIDTH == 64 ? 2 : 1;
+    // blocks an SM: 8 warps of a narrow head in 64 registers a thread, 4 times over, hide the loads' latency; the key warps'
+    // as many as their own registers allow, which keeps repair_rows' within them
+    static constexpr int kBlocks = KEY_WARPS > 1 ? (WIDTH == 32 ? 4 : WIDTH == 64 ? 3 : 2) : WIDTH == 32 ? 4 : WIDTH == 64 ? 2 : 1;
     static constexpr int kStageKeys = KEYS * KEY_WARPS;
     static constexpr int kTileBytes = kStageKeys * WIDTH * 2;  // the keys or the values of a stage
     static constexpr int kLoopBytes = STAGES * 2 * kTileBytes;
@@ -253,9 +254,8 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
                 else to.out[c] = static_cast<uint16_t>(pack16<BF16>(joined[i] * inverse, 0.0f) & 0xffff);
             }
             if (a.splits > 1 && lane == 0) to.part_sums[0] = top, to.part_sums[1] = total;
-            auto row_at = [&](int, int& its_token, int& its_head) { its_token = token, its_head = head; };
             if (isfinite(total) && !__all_sync(0xffffffffu, finite))
-                repair_rows<BF16>(a, b, 1, total == 0.0f ? 1 : 0, row_at, low, high, high, split, lane);
+                repair_rows<BF16, WIDTH>(a, b, 1, RowsAt{r, 0, first_head}, top, total, low, high, high, split);
         }
     } else {
         uint8_t* staged = smem + warp * 16 * WIDTH * 2;
@@ -295,16 +295,15 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
             }
         }
         if (__all_sync(0xffffffffu, finite[0] && finite[1])) return;
-        // rows whose output is not finite though their sum is, and those without a sum, from the votes of their quads
-        auto rows_of = [&](bool first, bool second) {
-            const uint32_t low8 = __ballot_sync(0xffffffffu, first), high8 = __ballot_sync(0xffffffffu, second);
-            uint32_t rows = 0;
-            for (int i = 0; i < 16; ++i) rows |= (((i < 8 ? low8 : high8) >> (i % 8 * 4)) & 15u) != 0 ? 1u << i : 0u;
-            return rows;
-        };
-        const uint32_t again = rows_of(!finite[0], !finite[1]), empty = rows_of(l[0] == 0.0f, l[1] == 0.0f);
-        auto row_at = [&](int i, int& token, int& head) { token = token_of(row_warp * 16 + i), head = head_of(row_warp * 16 + i); };
-        repair_rows<BF16>(a, b, again, empty, row_at, low, high, high, split, lane);
+        // rows whose output is not finite though their sum is, from the votes of their quads; a row's m and l to the row's lane
+        const uint32_t votes[2] = {__ballot_sync(0xffffffffu, !finite[0]), __ballot_sync(0xffffffffu, !finite[1])};
+        uint32_t again = 0;
+        for (int i = 0; i < 16; ++i) again |= (((i < 8 ? votes[0] : votes[1]) >> (i % 8 * 4)) & 15u) != 0 ? 1u << i : 0u;
+        const int from = lane % 8 * 4;
+        const float tops[2] = {__shfl_sync(0xffffffffu, m[0], from), __shfl_sync(0xffffffffu, m[1], from)};
+        const float sums[2] = {__shfl_sync(0xffffffffu, l[0], from), __shfl_sync(0xffffffffu, l[1], from)};
+        const RowsAt at{row_warp * 16, 0, first_head};
+        repair_rows<BF16, WIDTH>(a, b, again, at, lane < 8 ? tops[0] : tops[1], lane < 8 ? sums[0] : sums[1], low, high, high, split);
     }
 }
 

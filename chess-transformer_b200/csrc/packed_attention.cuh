@@ -151,78 +151,47 @@ FRY_DEVICE float4 load4(const uint16_t* from) {
     return make_float4(widen16<BF16>(words.x & 0xffff), widen16<BF16>(words.x >> 16), widen16<BF16>(words.y & 0xffff), widen16<BF16>(words.y >> 16));
 }
 
-// One row by its definition, by a warp: softmax over keys [low, high) in tiles of 32, lane i summing columns 4i to 4i + 3.
-// Slow, for rows that a value behind their last key has reached.
-template <bool BF16>
-FRY_DEVICE void recompute_row(const AttentionArgs& a, const RowBlock& b, int token, int head, int low, int high, int split, int lane) {
-    const uint16_t* q = a.q + (b.row + token) * a.q_row + head * a.q_head;
-    const uint16_t* k = a.k + b.k_base + (head / a.group) * a.k_head;
-    const bool mine = 4 * lane < a.width;
-    const uint16_t* v = a.v + b.v_base + (head / a.group) * a.v_head + (mine ? 4 * lane : 0);
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = low; j0 < high; j0 += 32) {
-        float s = -INFINITY;
-        if (j0 + lane < high) {
-            s = 0.0f;
-            const uint16_t* key = k + (j0 + lane) * a.k_row;
-#pragma unroll 4
-            for (int c = 0; c < a.width; c += 4) {
-                const float4 x = load4<BF16>(q + c), y = load4<BF16>(key + c);
-                s = __fmaf_rn(x.w, y.w, __fmaf_rn(x.z, y.z, __fmaf_rn(x.y, y.y, __fmaf_rn(x.x, y.x, s))));
-            }
-            s *= a.scale_log2;
-        }
-        const float top = fmaxf(m, warp_max(s)), base = top == -INFINITY ? 0.0f : top;
-        const float p = j0 + lane < high ? ex2_approx(s - base) : 0.0f, shrink = ex2_approx(m - base);
-        l = l * shrink + warp_sum(p);
-        m = top;
-        for (int i = 0; i < 4; ++i) o[i] *= shrink;
-#pragma unroll 8
-        for (int j = 0; j < 32; ++j) {
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            if (j0 + j >= high) continue;
-            const float4 x = load4<BF16>(v + (j0 + j) * a.v_row);
-            o[0] = __fmaf_rn(pj, x.x, o[0]), o[1] = __fmaf_rn(pj, x.y, o[1]), o[2] = __fmaf_rn(pj, x.z, o[2]), o[3] = __fmaf_rn(pj, x.w, o[3]);
-        }
-    }
-    const AttentionOut to = attention_out(a, split, b.row + token, head);
-    for (int i = 0; i < 4 && mine; ++i) {
-        if (a.splits > 1) to.part_out[4 * lane + i] = o[i];
-        else to.out[4 * lane + i] = static_cast<uint16_t>(pack16<BF16>(l == 0.0f ? 0.0f : o[i] / l, 0.0f) & 0xffff);
-    }
-    if (a.splits > 1 && lane == 0) to.part_sums[0] = m, to.part_sums[1] = l;
-}
-
 // What a column's values hold beside finite ones.
 constexpr uint32_t kHasInf = 1, kHasMinusInf = 2, kHasNan = 4;
 FRY_DEVICE uint32_t not_finite(float v) { return isfinite(v) ? 0u : isnan(v) ? kHasNan : v > 0.0f ? kHasInf : kHasMinusInf; }
 
-// Puts right the rows of a warp whose sums l are finite and whose outputs, written already, are not: bit i of `rows` for
-// row_at(i, token, head), of one key/value head, and of `empty` where l is 0. Their tile took the keys [low, taken); row i
-// sees those up to its limit, at most `high`. A value at its limit or behind that is not finite has been multiplied by 0
-// and made its column NaN. A row without such a value keeps its output, which is its own operands'. Of the others, a column
-// whose seen values are finite has to be summed again (recompute_row). One with a seen value that is not finite needs no
-// sum, since its probability is above 0: it is NaN, or the infinity of one sign that it holds. So an overflown value costs
-// its head the passes over the values below, and a row is summed again only in tiles that hold a column's first such value
-// (an infinity at the first of 4096 causal tokens, 8 heads of 128: 80 us a call, 71 without it, 69 ms with every row summed again).
-template <bool BF16, typename RowAt>
-FRY_DEVICE void repair_rows(const AttentionArgs& a, const RowBlock& b, uint32_t rows, uint32_t empty, RowAt row_at, int low, int high, int taken, int split,
-                            int lane) {
-    if (rows == 0) return;  // uniform across the warp
-    __syncwarp();           // the outputs are written
+// A warp's first row in its tile, and the token and head that the tile's first row has.
+struct RowsAt {
+    int row, token, head;
+};
+
+// Puts right the rows of a warp whose sums l are finite and whose outputs, written already, are not: bit i of `rows` for its
+// row i, whose m and l lane i holds. Their tile took the keys [low, taken); row i sees those up to its limit, at most
+// `high`. A value at its limit or behind that is not finite has been multiplied by 0 and made its column NaN. A row without
+// such a value keeps its output, which is its own operands'. Of the others' columns, one with a seen value that is not
+// finite needs no sum, since its probability is above 0: it is NaN, or the infinity of one sign that it holds. Those whose
+// seen values are finite are summed again, 16 rows and 32 columns at a time on mma.sync, with 0 for every value that is not
+// finite. So an overflown value costs its head passes over the values, and sums in the one tile of rows that holds a
+// column's first. 4096 causal tokens, 8 heads of 128, 72 us a call: with an infinity at the first token 83 us, at the last
+// 830, in one value of 500 1040 (a row at a time in scalars 69, 23 and 20 ms). Not inlined, and with b by value, so that the
+// kernels keep their registers.
+template <bool BF16, int WIDTH>
+__device__ __noinline__ void repair_rows(const AttentionArgs& a, RowBlock b, uint32_t rows, RowsAt at, float m, float l, int low, int high,
+                                         int taken, int split) {
+    __syncwarp();  // the outputs are written
+    const int lane = threadIdx.x & 31;
     int token, head;
     auto limit_of = [&](int i) {
-        row_at(i, token, head);
+        token = at.token + a.token_of(at.row + i), head = at.head + a.head_in_tile(at.row + i);
         return max(low, min(high, b.limit(token, a.causal)));
     };
     const int fewest = __reduce_min_sync(0xffffffffu, (rows >> lane) & 1 ? limit_of(lane) : INT_MAX);
-    row_at(__ffs(rows) - 1, token, head);
+    const int kv_head = at.head / a.group;
+    const uint16_t *keys = a.k + b.k_base + kv_head * a.k_head, *values = a.v + b.v_base + kv_head * a.v_head;
     const bool mine = 4 * lane < a.width;  // this lane's columns: 4 lane to 4 lane + 3
-    const uint16_t* v = a.v + b.v_base + (head / a.group) * a.v_head + (mine ? 4 * lane : 0);
+    auto values4 = [&](int j) {
+        const uint2 words = __ldg(reinterpret_cast<const uint2*>(values + j * a.v_row + (mine ? 4 * lane : 0)));
+        return make_float4(widen16<BF16>(words.x & 0xffff), widen16<BF16>(words.x >> 16), widen16<BF16>(words.y & 0xffff), widen16<BF16>(words.y >> 16));
+    };
     int last[4] = {-1, -1, -1, -1};  // the last key of [fewest, taken) whose value is not finite
 #pragma unroll 8
     for (int j = fewest; j < taken; ++j) {
-        const float4 x = load4<BF16>(v + j * a.v_row);
+        const float4 x = values4(j);
         if (!isfinite(x.x)) last[0] = j;
         if (!isfinite(x.y)) last[1] = j;
         if (!isfinite(x.z)) last[2] = j;
@@ -231,38 +200,123 @@ FRY_DEVICE void repair_rows(const AttentionArgs& a, const RowBlock& b, uint32_t 
     auto scan = [&](int from, int to, uint32_t (&holds)[4]) {
 #pragma unroll 8
         for (int j = from; j < to; ++j) {
-            const float4 x = load4<BF16>(v + j * a.v_row);
+            const float4 x = values4(j);
             holds[0] |= not_finite(x.x), holds[1] |= not_finite(x.y), holds[2] |= not_finite(x.z), holds[3] |= not_finite(x.w);
         }
     };
     uint32_t common[4] = {0, 0, 0, 0};  // of the keys that all these rows see
     bool scanned = false;
+    uint32_t sum_rows = 0, sum_lanes = 0, sums[4] = {0, 0, 0, 0};  // to be summed: rows, columns / 4; of lane's row, columns e of each 4
     for (; rows != 0; rows &= rows - 1) {
         const int i = __ffs(rows) - 1, limit = limit_of(i);
+        const bool empty = __shfl_sync(0xffffffffu, l, i) == 0.0f;  // no keys: zeros
         const AttentionOut to = attention_out(a, split, b.row + token, head);
-        auto write = [&](int e, float value) {
-            if (a.splits > 1) to.part_out[4 * lane + e] = value;
-            else to.out[4 * lane + e] = static_cast<uint16_t>(pack16<BF16>(value, 0.0f) & 0xffff);
-        };
-        if ((empty >> i) & 1) {
-            for (int e = 0; e < 4 && mine; ++e) write(e, 0.0f);
-            continue;
-        }
         bool reached[4], any = false;
-        for (int e = 0; e < 4; ++e) reached[e] = mine && last[e] >= limit, any = any || reached[e];
+        for (int e = 0; e < 4; ++e) reached[e] = mine && (empty || last[e] >= limit), any = any || reached[e];
         if (!__any_sync(0xffffffffu, any)) continue;
-        if (!scanned) scan(low, fewest, common);
-        scanned = true;
-        uint32_t holds[4] = {common[0], common[1], common[2], common[3]};
-        scan(fewest, limit, holds);
-        bool again = false;
-        for (int e = 0; e < 4; ++e) again = again || (reached[e] && holds[e] == 0);
-        if (__any_sync(0xffffffffu, again)) {
-            recompute_row<BF16>(a, b, token, head, low, limit, split, lane);
-            continue;
+        uint32_t holds[4] = {0, 0, 0, 0};
+        if (!empty) {
+            if (!scanned) scan(low, fewest, common);
+            scanned = true;
+            for (int e = 0; e < 4; ++e) holds[e] = common[e];
+            scan(fewest, limit, holds);
         }
-        for (int e = 0; e < 4; ++e)
-            if (reached[e]) write(e, holds[e] == kHasInf ? INFINITY : holds[e] == kHasMinusInf ? -INFINITY : NAN);
+        for (int e = 0; e < 4; ++e) {
+            const bool sum = reached[e] && holds[e] == 0 && !empty;
+            if (reached[e] && !sum) {
+                const float value = empty ? 0.0f : holds[e] == kHasInf ? INFINITY : holds[e] == kHasMinusInf ? -INFINITY : NAN;
+                if (a.splits > 1) to.part_out[4 * lane + e] = value;
+                else to.out[4 * lane + e] = static_cast<uint16_t>(pack16<BF16>(value, 0.0f) & 0xffff);
+            }
+            const uint32_t votes = __ballot_sync(0xffffffffu, sum);
+            if (votes) sum_rows |= 1u << i;
+            if (lane == i) sums[e] = votes;
+            sum_lanes |= votes;
+        }
+    }
+
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll 1
+    for (int first = 0; first < 32; first += 16) {
+        if (((sum_rows >> first) & 0xffffu) == 0) continue;
+        const uint16_t* q[2];
+        AttentionOut to[2];
+        int limit[2];
+        float base[2], inverse[2];
+        for (int half = 0; half < 2; ++half) {
+            const int i = first + g + 8 * half;
+            const float its_m = __shfl_sync(0xffffffffu, m, i), its_l = __shfl_sync(0xffffffffu, l, i);
+            limit[half] = low, base[half] = 0.0f, inverse[half] = a.splits > 1 ? 1.0f : 1.0f / its_l;
+            const bool summed = (sum_rows >> i) & 1;
+            const int its_limit = limit_of(summed ? i : __ffs(sum_rows) - 1);  // (the others take a summed row's query, and no keys)
+            q[half] = a.q + (b.row + token) * a.q_row + head * a.q_head;
+            to[half] = attention_out(a, split, b.row + token, head);
+            if (summed) limit[half] = its_limit, base[half] = its_m;
+        }
+        const int end = __reduce_max_sync(0xffffffffu, max(limit[0], limit[1]));
+#pragma unroll 1
+        for (int chunk = 0; chunk < WIDTH; chunk += 32) {
+            if (((sum_lanes >> (chunk / 4)) & 0xffu) == 0) continue;
+            float o[4][4] = {};
+#pragma unroll 1
+            for (int j0 = low; j0 < end; j0 += 16) {
+                // every load is made, from the last key and column where its own is behind them, so that all are in flight at once
+                auto key_at = [&](int j) { return j < end ? j : end - 1; };
+                uint16_t bits[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        bits[n][e] = __ldg(values + key_at(j0 + 8 * (e / 2) + 2 * t + e % 2) * a.v_row + min(chunk + 8 * n + g, a.width - 1));
+                // the products' K index, 8 of a head's columns a lane and 32 columns, is assigned alike for q and k
+                float s[2][4] = {};
+#pragma unroll
+                for (int w = 0; w < WIDTH; w += 32) {
+                    const bool inside = w + 8 * t < a.width;
+                    const int c = inside ? w + 8 * t : 0;
+                    uint4 x[2], k[2];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        x[half] = __ldg(reinterpret_cast<const uint4*>(q[half] + c));
+                        k[half] = __ldg(reinterpret_cast<const uint4*>(keys + key_at(j0 + 8 * half + g) * a.k_row + c));
+                        if (!inside) x[half] = k[half] = make_uint4(0, 0, 0, 0);
+                    }
+                    const uint32_t near[4] = {x[0].x, x[1].x, x[0].y, x[1].y}, far[4] = {x[0].z, x[1].z, x[0].w, x[1].w};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        mma16816<BF16>(s[n], near, k[n].x, k[n].y);
+                        mma16816<BF16>(s[n], far, k[n].z, k[n].w);
+                    }
+                }
+                uint32_t p[4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int j = j0 + 8 * n + 2 * t;
+                        const float even = ex2_approx_ftz(__fmaf_rn(s[n][2 * half], a.scale_log2, -base[half]));
+                        const float odd = ex2_approx_ftz(__fmaf_rn(s[n][2 * half + 1], a.scale_log2, -base[half]));
+                        p[2 * n + half] = pack16<BF16>(j < limit[half] ? even : 0.0f, j + 1 < limit[half] ? odd : 0.0f);
+                    }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!isfinite(widen16<BF16>(bits[n][e]))) bits[n][e] = 0;
+                    mma16816<BF16>(o[n], p, bits[n][0] | static_cast<uint32_t>(bits[n][1]) << 16, bits[n][2] | static_cast<uint32_t>(bits[n][3]) << 16);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int half = e >> 1, c = chunk + 8 * n + 2 * t + (e & 1);  // c % 4 == 2 t % 4 + e % 2
+                    const uint32_t even = __shfl_sync(0xffffffffu, sums[e & 1], first + g + 8 * half), odd = __shfl_sync(0xffffffffu, sums[2 + (e & 1)], first + g + 8 * half);
+                    if (!(((t % 2 == 0 ? even : odd) >> (c / 4)) & 1)) continue;
+                    if (a.splits > 1) to[half].part_out[c] = o[n][e];
+                    else to[half].out[c] = static_cast<uint16_t>(pack16<BF16>(o[n][e] * inverse[half], 0.0f) & 0xffff);
+                }
+        }
     }
 }
 

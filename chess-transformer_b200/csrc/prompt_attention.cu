@@ -401,12 +401,9 @@ __global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (Prompt
             }
             if (a.splits > 1 && live) to.part_sums[0] = m, to.part_sums[1] = total;
             // rows of finite sums whose outputs are not finite; the MMAs took the tile's keys in 16s
-            const uint32_t again = __ballot_sync(0xffffffffu, live && !finite && isfinite(total)), empty = __ballot_sync(0xffffffffu, total == 0.0f);
-            auto row_at = [&](int i, int& its_token, int& its_head) {
-                const int r = (warp & 3) * 32 + i;
-                its_token = t * tile + a.token_of(r), its_head = kv_head * a.group + head_tile * a.tile_heads + a.head_in_tile(r);
-            };
-            repair_rows<BF16>(a, b, again, empty, row_at, low, high, min(b.nk, low + (highs[t] - low + 15) / 16 * 16), split, lane);
+            const uint32_t again = __ballot_sync(0xffffffffu, live && !finite && isfinite(total));
+            const RowsAt at{(warp & 3) * 32, t * tile, kv_head * a.group + head_tile * a.tile_heads};
+            if (again) repair_rows<BF16, WIDTH>(a, b, again, at, m, total, low, high, min(b.nk, low + (highs[t] - low + 15) / 16 * 16), split);
         }
     }
     tc_fence_before();

@@ -148,3 +148,22 @@ def test_a_value_that_all_see_costs_little(queries, keys, heads, width, causal):
     print(f"{clean * 1e3:.1f} us, with the value {taken * 1e3:.1f} us")
     assert torch.isposinf(call()[:, :, 5]).all()
     assert taken <= 10 * clean + 0.1
+
+
+@pytest.mark.parametrize("queries, heads, kv_heads, width", [([4096], 8, 8, 128), ([4096], 8, 2, 64), ([1024] * 4, 8, 8, 64), ([64] * 64, 8, 8, 32)])
+def test_a_value_that_only_the_last_sees_costs_little(queries, heads, kv_heads, width):
+    """The rows before it in its tile are summed again: 16 rows by 32 columns of a warp at once, by width * 16 + 32 * 16 products
+    a key, which is a few of the passes that a warp of the same tile makes anyway, and the rest of the call does not wait."""
+    normal = lambda n: torch.randn(sum(queries), n, width, device="cuda").half()  # noqa: E731
+    q, k, v, at = normal(heads), normal(kv_heads), normal(kv_heads), offsets(queries)
+    call = lambda: ops.packed_attention(q, k, v, at, at)  # noqa: E731
+    clean, right = elapsed(call), call()
+    last = at[1:].long() - 1
+    v[last, :, 5] = math.nan
+    taken, found = elapsed(call), call()
+    print(f"{clean * 1e3:.1f} us, with the value {taken * 1e3:.1f} us")
+    assert torch.isnan(found[last, :, 5]).all()
+    found[last, :, 5] = right[last, :, 5]
+    # the sums again are of the same rounded factors, in another order and with probabilities against the last maximum
+    assert (found.double() - right.double()).abs().max() <= 4 * 2.0 ** -11 * v[torch.isfinite(v)].abs().max()
+    assert taken <= 20 * clean + 0.1
