@@ -9,6 +9,8 @@
 // pair, low's block against up[a]'s rows. slot_adapter gives a slot's adapter (-1: none) and tile_slots a tile's slots.
 //
 // low is rounded to fp16 (at most half a step a value, 2^-11 of it, as rounding the output costs); its sums are fp32.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "rowops.cuh"
@@ -40,15 +42,27 @@ FRY_DEVICE void widen_pairs(const uint4& raw, uint32_t* pairs) {
     }
 }
 
+// c += a b^T, 16 rows by 8 columns over 32 int8 values
+FRY_DEVICE void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // A block's product of up to 32 rows of x, in `groups` of 16 (rows below `low` or from `high` on count as 0), with TILES * 8
 // rows of w (those from `columns` on count as 0), K long both: the warps take runs of K in turn and leave their sums in
 // partial [kThinWarps][kThinRows][TILES * 8]. A lane's MMA fragments come from 16-byte loads: of each run of K the four
 // lanes of a quad read 16 (of int8 x against fp16 w, 16 and 32) bytes each, and the MMA's K index is assigned to what a lane
 // holds, alike for x and w (a sum over K may take it in any order). Each block reads its x and w once, and the loads bound
 // it: what a warp has in flight (kAhead runs), blocks an SM, and the search and the first load before them. Warps that
-// share K rather than rows read each weight once a block (4333 rows of 2048, rank 32: 47.6 -> 17.3 us).
+// share K rather than rows read each weight once a block (4333 rows of 2048, rank 32: 47.6 -> 17.3 us). The sums are fp32,
+// of int8 x and w exact int32.
+template <bool X_INT8, bool W_INT8>
+using ThinSum = std::conditional_t<X_INT8 && W_INT8, int, float>;
 template <bool X_INT8, bool W_INT8, int TILES, int GROUPS>
-FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
+FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K,
+                                ThinSum<X_INT8, W_INT8>* partial) {
+    static_assert(X_INT8 || !W_INT8, "int8 weights take int8 rows");
     constexpr int kSteps = X_INT8 ? 4 : 2;          // MMA K steps of 16 a run
     constexpr int kLane = kSteps * 4;               // K values a lane holds of a run
     constexpr int kRun = 4 * kLane;
@@ -59,7 +73,11 @@ FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high,
     const uint8_t* x_lane = static_cast<const uint8_t*>(x) + (static_cast<size_t>(first_row + g) * K + t * kLane) * (X_INT8 ? 1 : 2);
     const uint8_t* w_lane = static_cast<const uint8_t*>(w) + (static_cast<size_t>(g) * K + t * kLane) * (W_INT8 ? 1 : 2);
     const size_t x_step = static_cast<size_t>(K) * 8 * (X_INT8 ? 1 : 2), w_step = static_cast<size_t>(K) * 8 * (W_INT8 ? 1 : 2);
-    float sums[GROUPS][TILES][4] = {};
+    using Sum = ThinSum<X_INT8, W_INT8>;
+    struct alignas(8) Pair {
+        Sum first, second;
+    };
+    Sum sums[GROUPS][TILES][4] = {};
     for (int run = warp * kRun; run < K; run += kThinWarps * kRun * kAhead) {
         uint4 raw[kAhead][GROUPS][2], weight[kAhead][TILES][kLoads];
 #pragma unroll
@@ -85,22 +103,35 @@ FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high,
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            uint32_t b[TILES][2 * kSteps];
+            if constexpr (W_INT8) {  // both int8: two steps of 32 a run
 #pragma unroll
-            for (int n = 0; n < TILES; ++n)
+                for (int i = 0; i < GROUPS; ++i) {
+                    if (i >= groups) break;
+                    const uint4 &a0 = raw[u][i][0], &a1 = raw[u][i][1];
 #pragma unroll
-                for (int h = 0; h < kLoads; ++h) widen_pairs<W_INT8>(weight[u][n][h], b[n] + 4 * h);
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                if (i >= groups) break;
-                uint32_t a[2][2 * kSteps];
-                widen_pairs<X_INT8>(raw[u][i][0], a[0]);
-                widen_pairs<X_INT8>(raw[u][i][1], a[1]);
+                    for (int n = 0; n < TILES; ++n) {
+                        mma_s8(sums[i][n], a0.x, a1.x, a0.y, a1.y, weight[u][n][0].x, weight[u][n][0].y);
+                        mma_s8(sums[i][n], a0.z, a1.z, a0.w, a1.w, weight[u][n][0].z, weight[u][n][0].w);
+                    }
+                }
+            } else {
+                uint32_t b[TILES][2 * kSteps];
 #pragma unroll
                 for (int n = 0; n < TILES; ++n)
 #pragma unroll
-                    for (int s = 0; s < kSteps; ++s)
-                        mma_f16(sums[i][n], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[n][2 * s], b[n][2 * s + 1]);
+                    for (int h = 0; h < kLoads; ++h) widen_pairs<false>(weight[u][n][h], b[n] + 4 * h);
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) {
+                    if (i >= groups) break;
+                    uint32_t a[2][2 * kSteps];
+                    widen_pairs<X_INT8>(raw[u][i][0], a[0]);
+                    widen_pairs<X_INT8>(raw[u][i][1], a[1]);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                        for (int s = 0; s < kSteps; ++s)
+                            mma_f16(sums[i][n], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[n][2 * s], b[n][2 * s + 1]);
+                }
             }
         }
     }
@@ -111,24 +142,24 @@ FRY_DEVICE void thin_product_of(const void* x, int first_row, int low, int high,
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
-                *reinterpret_cast<float2*>(partial + ((warp * kThinRows + i * 16 + half * 8 + g) * TILES + n) * 8 + 2 * t) =
-                    make_float2(sums[i][n][2 * half], sums[i][n][2 * half + 1]);
+                *reinterpret_cast<Pair*>(partial + ((warp * kThinRows + i * 16 + half * 8 + g) * TILES + n) * 8 + 2 * t) = {sums[i][n][2 * half], sums[i][n][2 * half + 1]};
     }
 }
 template <bool X_INT8, bool W_INT8, int TILES>
-FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K, float* partial) {
+FRY_DEVICE void thin_product(const void* x, int first_row, int low, int high, int groups, const void* w, int columns, int K,
+                             ThinSum<X_INT8, W_INT8>* partial) {
     if (groups == 1) thin_product_of<X_INT8, W_INT8, TILES, 1>(x, first_row, low, high, 1, w, columns, K, partial);
     else thin_product_of<X_INT8, W_INT8, TILES, kThinRows / 16>(x, first_row, low, high, groups, w, columns, K, partial);
 }
 // The warps' sums of columns [column, column + COUNT) of a row, in the order of the warps.
-template <int TILES, int COUNT>
-FRY_DEVICE void thin_total(const float* partial, int row, int column, float (&total)[COUNT]) {
+template <int TILES, typename Sum, int COUNT>
+FRY_DEVICE void thin_total(const Sum* partial, int row, int column, Sum (&total)[COUNT]) {
 #pragma unroll
-    for (int e = 0; e < COUNT; ++e) total[e] = 0.0f;
+    for (int e = 0; e < COUNT; ++e) total[e] = 0;
 #pragma unroll
     for (int q = 0; q < kThinWarps; ++q)
 #pragma unroll
-        for (int e = 0; e < COUNT; ++e) total[e] = __fadd_rn(total[e], partial[(q * kThinRows + row) * TILES * 8 + column + e]);
+        for (int e = 0; e < COUNT; ++e) total[e] += partial[(q * kThinRows + row) * TILES * 8 + column + e];
 }
 
 // low of 32 rows of a slot and up to TILES * 8 columns of the rank.
@@ -195,7 +226,9 @@ __global__ void __launch_bounds__(kThinWarps * 32, TILES == 1 ? 3 : TILES <= 4 ?
 template <bool INT8>
 __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const AdapterArgs p, const GemmArgs args, const void* weight, int M, int N, int K) {
     constexpr int kTiles = 2, kColumns = kTiles * 8;
-    extern __shared__ __align__(16) float partial[];
+    using Sum = ThinSum<INT8, INT8>;
+    extern __shared__ __align__(16) uint8_t thin_smem[];
+    Sum* partial = reinterpret_cast<Sum*>(thin_smem);
     const int slots = packed_slots(M, p.tile_rows, p.requests);
     const int n0 = blockIdx.x * kColumns, columns = min(kColumns, N - n0);
     thin_product<INT8, INT8, kTiles>(p.x, 0, 0, M, (M + 15) / 16, static_cast<const uint8_t*>(weight) + static_cast<size_t>(n0) * K * (INT8 ? 1 : 2), columns, K,
@@ -205,7 +238,8 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
     for (int i = threadIdx.x; i < M * kColumns / 2; i += kThinWarps * 32) {
         const int m = i / (kColumns / 2), c = i % (kColumns / 2) * 2, n = n0 + c;
         if (c >= columns) continue;
-        float total[2], added[2] = {0.0f, 0.0f};
+        Sum total[2];
+        float added[2] = {0.0f, 0.0f};
         thin_total<kTiles>(partial, m, c, total);
         // (rows of offsets that descend may have no slot written)
         const int slot = p.row_slot[m], adapter = slot >= 0 && slot < slots ? p.slot_adapter[slot] : -1;
@@ -228,7 +262,7 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
         for (int h = 0; h < 2; ++h) {
             const float b = args.bias ? h2f_bits(args.bias[n + h]) : 0.0f;
             // as the GEMM's epilogues: the scales and bias then the adapter (int8), or the adapter in the sums then the bias
-            value[h] = INT8 ? __fadd_rn(__fmaf_rn(__fmul_rn(total[h], args.x_scale[m]), args.w_scale[n + h], b), added[h])
+            value[h] = INT8 ? __fadd_rn(__fmaf_rn(__fmul_rn(static_cast<float>(total[h]), args.x_scale[m]), args.w_scale[n + h], b), added[h])
                             : __fadd_rn(__fadd_rn(total[h], added[h]), b);
         }
         const size_t at = static_cast<size_t>(m) * N + n;

@@ -79,9 +79,8 @@ int fry_int8_linear_normed(const uint16_t* x, const uint16_t* gain, float eps, c
  * request), and
  *   out[m] = fp16((fma(acc * x_scale, weight_scale, bias) + (x_scale x[m] down[a]^T) up[a]^T) + residual[m])
  * down fp16 [adapters, rank, K], up fp16 [adapters, N, rank] (a scale of the adapter is the caller's, in either); the
- * adapters' sums fp32, x down^T rounded to fp16 between the two products (beyond 65504 it is infinite); up to 32 rows acc
- * is summed in fp32 too. bias and residual fp16, either NULL: none. An
- * adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids out of range are recorded in the device
+ * adapters' sums fp32, x down^T rounded to fp16 between the two products (beyond 65504 it is infinite); acc is the
+ * exact int32 sum. bias and residual fp16, either NULL: none. An adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids out of range are recorded in the device
  * status (code 7, where = the request): ids count as -1, rows of such offsets hold unspecified values. rank a multiple of 8
  * up to 128, N of 8, K of 16, adapters * N below 2^31, M and requests below 2^24; out overlaps no input but residual;
  * x, weight, down, up, residual, out and workspace 16-byte aligned. workspace: of fry_int8_adapter_linear_workspace_bytes;
