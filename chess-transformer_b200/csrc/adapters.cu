@@ -8,7 +8,10 @@
 // (tile, request) pair has the tile's rows, those of other requests zero, and the GEMM takes one step of rank columns a
 // pair, low's block against up[a]'s rows. slot_adapter gives a slot's adapter (-1: none) and tile_slots a tile's slots.
 //
-// low is rounded to fp16 (at most half a step a value, 2^-11 of it, as rounding the output costs); its sums are fp32.
+// low's sums are fp32. The GEMM takes them rounded to fp16, as rounding the output costs: off by 2^-11 of a value from 2^-14
+// on, by 2^-25 below that. Eight of a row's that hold a finite value beyond fp16 (65504) are kept in fp32 (low32), and
+// kBeyondFp16 in the first's place makes the row's sums NaN, which take_sums_again makes good. Up to 32 rows take no GEMM
+// and keep all of low in fp32.
 #include <type_traits>
 
 #include "common.cuh"
@@ -19,6 +22,12 @@
 namespace fry {
 
 constexpr int kThinRows = 32, kThinWarps = 8;  // rows of x a block takes; its warps share K
+constexpr uint16_t kBeyondFp16 = 0x7e2a;       // a NaN that no conversion gives (theirs is 0x7fff)
+
+FRY_DEVICE void load8(const float* from, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 
 // 16 bytes as fp16 pairs: 8 fp16 values, or 16 int8 values. int8 widens exactly: a byte with its sign bit flipped in the
 // low bits of 1024.0's fp16 pattern is 1024 + 128 + value.
@@ -181,8 +190,8 @@ __global__ void __launch_bounds__(kThinWarps * 32, TILES == 1 ? 3 : TILES <= 4 ?
         if (slot == 0)  // one block records the requests that are not in range, for all
             for (int s = threadIdx.x; s < p.requests; s += kThinWarps * 32)
                 if (rows.bad(s + 1) || p.ids[s] < -1 || p.ids[s] >= p.adapters) record_error(kBadOffsets, s);
-        if (p.row_slot)
-            for (int m = first + threadIdx.x; m < last; m += kThinWarps * 32) p.row_slot[m] = known ? slot : -1;
+        if (p.row_adapter)
+            for (int m = first + threadIdx.x; m < last; m += kThinWarps * 32) p.row_adapter[m] = known ? adapter : -1;
         if (threadIdx.x == 0) {
             p.slot_adapter[slot] = known ? adapter : -1;
             if (first < last && first == tile_first) p.tile_slots[tile].x = slot;
@@ -207,13 +216,25 @@ __global__ void __launch_bounds__(kThinWarps * 32, TILES == 1 ? 3 : TILES <= 4 ?
                 float total[8];
                 thin_total<TILES>(partial, row - group_first * 16, unit * 8, total);
                 const float scale = INT8 ? p.x_scale[m] : 1.0f;
+                bool beyond = false;  // finite, and infinite in fp16
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    total[e] = __fmul_rn(total[e], scale);
+                    beyond = beyond || (fabsf(total[e]) >= 65520.0f && isfinite(total[e]));
+                }
+                if (beyond || p.row_adapter) {
+                    float4* kept = reinterpret_cast<float4*>(p.low32 + static_cast<size_t>(m) * p.rank + rank_first + unit * 8);
+                    kept[0] = make_float4(total[0], total[1], total[2], total[3]), kept[1] = make_float4(total[4], total[5], total[6], total[7]);
+                }
                 uint32_t* words = reinterpret_cast<uint32_t*>(&packed);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) words[e] = pack_half2_rn(__fmul_rn(total[2 * e], scale), __fmul_rn(total[2 * e + 1], scale));
+                for (int e = 0; e < 4; ++e) words[e] = pack_half2_rn(total[2 * e], total[2 * e + 1]);
+                if (beyond) words[0] = kBeyondFp16;
             }
+            if (p.row_adapter) continue;
             *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * p.rank + unit * 8) = packed;
         }
-    } else {  // none of its rows: zeros
+    } else if (!p.row_adapter) {  // none of its rows: zeros
         for (int i = threadIdx.x; i < kThinRows * units; i += kThinWarps * 32)
             *reinterpret_cast<uint4*>(out + static_cast<size_t>(i / units) * p.rank + i % units * 8) = make_uint4(0, 0, 0, 0);
     }
@@ -229,11 +250,10 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
     using Sum = ThinSum<INT8, INT8>;
     extern __shared__ __align__(16) uint8_t thin_smem[];
     Sum* partial = reinterpret_cast<Sum*>(thin_smem);
-    const int slots = packed_slots(M, p.tile_rows, p.requests);
     const int n0 = blockIdx.x * kColumns, columns = min(kColumns, N - n0);
     thin_product<INT8, INT8, kTiles>(p.x, 0, 0, M, (M + 15) / 16, static_cast<const uint8_t*>(weight) + static_cast<size_t>(n0) * K * (INT8 ? 1 : 2), columns, K,
                                      partial);
-    grid_dependency_start();  // low and row_slot are made
+    grid_dependency_start();  // low32 and row_adapter are made
     __syncthreads();
     for (int i = threadIdx.x; i < M * kColumns / 2; i += kThinWarps * 32) {
         const int m = i / (kColumns / 2), c = i % (kColumns / 2) * 2, n = n0 + c;
@@ -241,14 +261,13 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
         Sum total[2];
         float added[2] = {0.0f, 0.0f};
         thin_total<kTiles>(partial, m, c, total);
-        // (rows of offsets that descend may have no slot written)
-        const int slot = p.row_slot[m], adapter = slot >= 0 && slot < slots ? p.slot_adapter[slot] : -1;
+        const int adapter = p.row_adapter[m];  // (rows of offsets that descend may have none written)
         if (adapter >= 0 && adapter < p.adapters) {
-            const uint4* low = reinterpret_cast<const uint4*>(p.low + (static_cast<size_t>(slot) * p.tile_rows + m % p.tile_rows) * p.rank);
+            const float* low = p.low32 + static_cast<size_t>(m) * p.rank;
             const uint4* up = reinterpret_cast<const uint4*>(p.up + (static_cast<size_t>(adapter) * N + n) * p.rank);
             for (int j = 0; j < p.rank / 8; ++j) {
                 float l[8], u[8];
-                unpack8(low[j], l);
+                load8(low + 8 * j, l);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     unpack8(__ldg(up + h * (p.rank / 8) + j), u);
@@ -274,23 +293,24 @@ __global__ void __launch_bounds__(kThinWarps * 32) adapter_thin_kernel(const Ada
     }
 }
 
-// x . y over `count` fp16 values, a multiple of 8, both on 16 bytes.
-FRY_DEVICE float dot16(const uint16_t* x, const uint16_t* y, int count) {
+// Row m's low, in its slot, times up[.., n] of its adapter.
+FRY_DEVICE float low_up(const AdapterArgs& p, const uint16_t* low, const uint16_t* up, int m) {
     float sum = 0.0f;
-    for (int k = 0; k < count; k += 8) {
-        float a[8], b[8];
-        unpack8(*reinterpret_cast<const uint4*>(x + k), a);
-        unpack8(*reinterpret_cast<const uint4*>(y + k), b);
+    for (int j = 0; j < p.rank; j += 8) {
+        float l[8], u[8];
+        if (low[j] == kBeyondFp16) load8(p.low32 + static_cast<size_t>(m) * p.rank + j, l);
+        else unpack8(*reinterpret_cast<const uint4*>(low + j), l);
+        unpack8(__ldg(reinterpret_cast<const uint4*>(up + j)), u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __fmaf_rn(a[e], b[e], sum);
+        for (int e = 0; e < 8; ++e) sum = __fmaf_rn(l[e], u[e], sum);
     }
     return sum;
 }
 
-// A sum that is not finite stands where no other request of the tile has an adapter that is not finite in its column: it is
-// the row's own then. The others are the row's x . w (kEpiAdapterF16; a warp's 32 x 16 of them on mma.sync, its fragments as in
+// A sum that is not finite stands where no other request of the tile has an adapter that is not finite in its column and all
+// of the row's low is in fp16: it is the row's own then. The others are the row's x . w (kEpiAdapterF16; a warp's 32 x 16 of them on mma.sync, its fragments as in
 // thin_product_of) plus low . up of its own request. 3744 rows through 2048 x 2048, rank 32, 50 us a call: 86 us with an x
-// that is not finite in every row, 1.08 ms with a quarter of the requests on a NaN adapter; summed again in scalars, 79 ms.
+// that is not finite in every row, 1.08 ms with a quarter of the requests on a NaN adapter or with all of low beyond fp16; summed again in scalars, 79 ms.
 template <int EPI>
 __device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, int column, uint32_t* sums) {
     const int lane = threadIdx.x & 31, first_row = m - lane, tile_rows = p.adapters.tile_rows, tile = first_row / tile_rows, rank = p.adapters.rank;
@@ -317,6 +337,10 @@ __device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, in
         const uint32_t votes = __ballot_sync(0xffffffffu, found);
         if (!mine) reached |= (votes | votes >> 16) & 0xffffu;
     }
+    const uint16_t* low = p.adapters.low + (static_cast<size_t>(own_slot < 0 ? 0 : own_slot) * tile_rows + m % tile_rows) * rank;
+    if (bad && own_slot >= 0)
+        for (int j = 0; j < rank; j += 8)
+            if (low[j] == kBeyondFp16) reached = 0xffffu;
     const uint32_t again = bad & reached;
     if (!__any_sync(0xffffffffu, again != 0)) return;
 
@@ -360,8 +384,7 @@ __device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, in
         }
         if (!((again >> e) & 1)) continue;
         if (own_slot >= 0)
-            sum += dot16(p.adapters.low + (static_cast<size_t>(own_slot) * tile_rows + m % tile_rows) * rank,
-                         p.adapters.up + (static_cast<size_t>(own_adapter) * p.N + column + e) * rank, rank);
+            sum += low_up(p.adapters, low, p.adapters.up + (static_cast<size_t>(own_adapter) * p.N + column + e) * rank, m);
         sums[e] = __float_as_uint(sum);
     }
 }
@@ -402,11 +425,13 @@ int slot_rows(int kind, int M, int N) { return M <= kThinMost ? kThinRows : adap
 AdapterWorkspace::AdapterWorkspace(int kind, int M, int N, int requests, int rank) : tile_rows(slot_rows(kind, M, N)) {
     const size_t tiles = (static_cast<size_t>(M) + tile_rows - 1) / tile_rows;
     auto up = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    const bool thin = M <= kThinMost;
     slots = packed_slots(M, tile_rows, requests);
-    tile_slots = up(slots * tile_rows * rank * 2);
+    tile_slots = thin ? 0 : up(slots * tile_rows * rank * 2);
     slot_adapter = tile_slots + up(tiles * sizeof(int2));
-    row_slot = slot_adapter + up(slots * sizeof(int32_t));
-    total = row_slot + (M <= kThinMost ? up(M * sizeof(int32_t)) : 0);
+    low32 = slot_adapter + up(slots * sizeof(int32_t));
+    row_adapter = low32 + up(static_cast<size_t>(M) * rank * sizeof(float));
+    total = row_adapter + (thin ? up(M * sizeof(int32_t)) : 0);
 }
 
 cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& p, const void* weight, int M, int N, int K, void* workspace, cudaStream_t stream,
@@ -418,7 +443,8 @@ cudaError_t adapter_linear(int kind, GemmArgs& gemm_args, AdapterArgs& p, const 
     p.tile_slots = reinterpret_cast<int2*>(base + layout.tile_slots);
     p.slot_adapter = reinterpret_cast<int32_t*>(base + layout.slot_adapter);
     const bool thin = M <= kThinMost;
-    if (thin) p.row_slot = reinterpret_cast<int32_t*>(base + layout.row_slot);
+    p.low32 = reinterpret_cast<float*>(base + layout.low32);
+    if (thin) p.row_adapter = reinterpret_cast<int32_t*>(base + layout.row_adapter);
     const cudaError_t status = kind == 0 ? low_rank_rows<true>(p, M, K, stream) : low_rank_rows<false>(p, M, K, stream);
     if (status != cudaSuccess) return status;
     if (thin) return kind == 0 ? launch_thin<true>(p, gemm_args, weight, M, N, K, stream) : launch_thin<false>(p, gemm_args, weight, M, N, K, stream);

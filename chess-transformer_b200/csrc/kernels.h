@@ -77,12 +77,13 @@ struct AdapterArgs {
     uint16_t* low = nullptr;
     int2* tile_slots = nullptr;
     int32_t* slot_adapter = nullptr;
-    int32_t* row_slot = nullptr;           // few rows: a row's slot (-1: no adapter)
+    float* low32 = nullptr;                // x down^T of row m in fp32 [M, rank]: of few rows all, else the eights of it beyond fp16
+    int32_t* row_adapter = nullptr;        // few rows: a row's adapter (-1: none), and low is not made
 };
 // The workspace: low first, then the others where these say, each 256-byte aligned.
 struct AdapterWorkspace {
     int tile_rows;
-    size_t slots, tile_slots, slot_adapter, row_slot, total;
+    size_t slots, tile_slots, slot_adapter, low32, row_adapter, total;
     AdapterWorkspace(int kind, int M, int N, int requests, int rank);
     int64_t low_rows() const { return static_cast<int64_t>(slots) * tile_rows; }
 };

@@ -317,7 +317,9 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     x W^T + bias + residual, plus (x down[a]^T) up[a]^T for the rows offsets[s] to offsets[s + 1] of request s, a = ids[s].
     x [..., K], weight [N, K] as nn.Linear holds it, down [adapters, rank, K], up [adapters, N, rank]; offsets [requests + 1]
     and ids [requests] int32 on the device; rows of no request and those of ids -1 have no adapter. rank a multiple of 8 up
-    to 128 (pad smaller ones with zeros), N and K multiples of 8. No backward pass."""
+    to 128 (pad smaller ones with zeros), N and K multiples of 8. Sums are fp32; from 33 rows on x down^T is rounded to fp16
+    between the two products (off by 2^-11 of a value, by 2^-25 below 2^-14; beyond 65504 it stays fp32, which is slower). No
+    backward pass."""
     index, shapes, operands = _adapter_operands("adapter_linear", x, weight, bias, residual, down, up, offsets, ids, torch.float16)
     M, N, _, requests, _, rank = shapes
     out = x.new_empty(*x.shape[:-1], N)

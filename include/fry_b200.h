@@ -78,13 +78,14 @@ int fry_int8_linear_normed(const uint16_t* x, const uint16_t* gain, float eps, c
  * a = ids[s] (offsets int32 [requests + 1] ascending, ids int32 [requests], both on the device; -1: none, as for rows of no
  * request), and
  *   out[m] = fp16((fma(acc * x_scale, weight_scale, bias) + (x_scale x[m] down[a]^T) up[a]^T) + residual[m])
- * down fp16 [adapters, rank, K], up fp16 [adapters, N, rank] (a scale of the adapter is the caller's, in either); the
- * adapters' sums fp32, x down^T rounded to fp16 between the two products (beyond 65504 it is infinite); acc is the
- * exact int32 sum. bias and residual fp16, either NULL: none. An adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids out of range are recorded in the device
- * status (code 7, where = the request): ids count as -1, rows of such offsets hold unspecified values. rank a multiple of 8
- * up to 128, N of 8, K of 16, adapters * N below 2^31, M and requests below 2^24; out overlaps no input but residual;
- * x, weight, down, up, residual, out and workspace 16-byte aligned. workspace: of fry_int8_adapter_linear_workspace_bytes;
- * calls whose work overlaps on the GPU need workspaces of their own. No reference counterpart. */
+ * down fp16 [adapters, rank, K], up fp16 [adapters, N, rank] (a scale of the adapter is the caller's, in either); acc is the
+ * exact int32 sum, the adapters' sums are fp32. Up to 32 rows x down^T is fp32 too; more rows take it rounded to fp16 (off by
+ * 2^-11 of a value, by 2^-25 below 2^-14), where it lies beyond 65504 eight values at a time in fp32, which is slower. bias
+ * and residual fp16, either NULL: none. An adapter reaches its own requests' rows alone, whatever it holds. Offsets or ids
+ * out of range are recorded in the device status (code 7, where = the request): ids count as -1, rows of such offsets hold
+ * unspecified values. rank a multiple of 8 up to 128, N of 8, K of 16, adapters * N below 2^31, M and requests below 2^24;
+ * out overlaps no input but residual; x, weight, down, up, residual, out and workspace 16-byte aligned. workspace: of
+ * fry_int8_adapter_linear_workspace_bytes; calls whose work overlaps on the GPU need workspaces of their own. No reference counterpart. */
 size_t fry_int8_adapter_linear_workspace_bytes(int M, int N, int requests, int rank);
 int fry_int8_adapter_linear(const int8_t* x, const float* x_scale, const int8_t* weight, const float* weight_scale, const uint16_t* bias,
                             const uint16_t* residual, const uint16_t* down, const uint16_t* up, const int32_t* offsets, const int32_t* ids,
