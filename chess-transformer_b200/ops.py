@@ -224,7 +224,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
     _call(library().fry_packed_attention, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
           k_offsets.data_ptr(), rows, key_rows, sequences, heads, kv_heads, width, q_row, q_head, k_row, k_head, v_row, v_head,
-          width ** -0.5 if scale is None else scale, causal, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
+          (width or 1) ** -0.5 if scale is None else scale, causal, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
     return out
 
 
@@ -254,7 +254,7 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
     _call(library().fry_cached_attention, index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lengths.data_ptr(), sequences,
           capacity, heads, kv_heads, width, q_row, q_head, k_sequence, k_row, k_head, v_sequence, v_row, v_head,
-          width ** -0.5 if scale is None else scale, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
+          (width or 1) ** -0.5 if scale is None else scale, dtype is torch.bfloat16, workspace.data_ptr() if size else None, size)
     return out
 
 
