@@ -34,7 +34,7 @@ struct RowsShape {
     static constexpr int kMaxThreads = (KEY_WARPS > 1 ? KEY_WARPS : kMaxRowWarps) * 32;
     // blocks an SM: 8 warps of a narrow head in 64 registers a thread, 4 times over, hide the loads' latency; the key warps'
     // as many as their own registers allow, which keeps repair_rows' within them
-    static constexpr int kBlocks = KEY_WARPS > 1 ? (WIDTH == 32 ? 4 : WIDTH == 64 ? 3 : 2) : WIDTH == 32 ? 4 : WIDTH == 64 ? 2 : 1;
+    static constexpr int kBlocks = KEY_WARPS > 1 ? (WIDTH == 128 ? 2 : 4) : WIDTH == 32 ? 4 : WIDTH == 64 ? 2 : 1;
     static constexpr int kStageKeys = KEYS * KEY_WARPS;
     static constexpr int kTileBytes = kStageKeys * WIDTH * 2;  // the keys or the values of a stage
     static constexpr int kLoopBytes = STAGES * 2 * kTileBytes;

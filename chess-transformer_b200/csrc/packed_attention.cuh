@@ -168,7 +168,7 @@ struct RowsAt {
 // seen values are finite are summed again, 16 rows and 32 columns at a time on mma.sync, with 0 for every value that is not
 // finite. So an overflown value costs its head passes over the values, and sums in the one tile of rows that holds a
 // column's first. 4096 causal tokens, 8 heads of 128, 72 us a call: with an infinity at the first token 83 us, at the last
-// 830, in one value of 500 1040 (a row at a time in scalars 69, 23 and 20 ms). Not inlined, and with b by value, so that the
+// 1020, in one value of 500 1050 (a row at a time in scalars 69, 23 and 20 ms). Not inlined, and with b by value, so that the
 // kernels keep their registers.
 template <bool BF16, int WIDTH>
 __device__ __noinline__ void repair_rows(const AttentionArgs& a, RowBlock b, uint32_t rows, RowsAt at, float m, float l, int low, int high,
@@ -270,7 +270,7 @@ __device__ __noinline__ void repair_rows(const AttentionArgs& a, RowBlock b, uin
                         bits[n][e] = __ldg(values + key_at(j0 + 8 * (e / 2) + 2 * t + e % 2) * a.v_row + min(chunk + 8 * n + g, a.width - 1));
                 // the products' K index, 8 of a head's columns a lane and 32 columns, is assigned alike for q and k
                 float s[2][4] = {};
-#pragma unroll
+#pragma unroll 1
                 for (int w = 0; w < WIDTH; w += 32) {
                     const bool inside = w + 8 * t < a.width;
                     const int c = inside ? w + 8 * t : 0;
