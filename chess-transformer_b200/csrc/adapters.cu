@@ -7,6 +7,8 @@
 // A tile of the GEMM may hold rows of several requests. low is therefore laid out by slots (segments.cuh): the block of a
 // (tile, request) pair has the tile's rows, those of other requests zero, and the GEMM takes one step of rank columns a
 // pair, low's block against up[a]'s rows. slot_adapter gives a slot's adapter (-1: none) and tile_slots a tile's slots.
+// This suits requests of many rows. One row a request costs a step and a block of low each, shared adapter or not: 2048 x 2048,
+// rank 16, 32 single rows (the thin kernel) 16 us, 33 26, 64 35, 128 52, 256 57, 1024 124.
 //
 // low's sums are fp32. The GEMM takes them rounded to fp16, as rounding the output costs: off by 2^-11 of a value from 2^-14
 // on, by 2^-25 below that. Eight of a row's that hold a finite value beyond fp16 (65504) are kept in fp32 (low32), and
@@ -308,9 +310,10 @@ FRY_DEVICE float low_up(const AdapterArgs& p, const uint16_t* low, const uint16_
 }
 
 // A sum that is not finite stands where no other request of the tile has an adapter that is not finite in its column and all
-// of the row's low is in fp16: it is the row's own then. The others are the row's x . w (kEpiAdapterF16; a warp's 32 x 16 of them on mma.sync, its fragments as in
-// thin_product_of) plus low . up of its own request. 3744 rows through 2048 x 2048, rank 32, 50 us a call: 86 us with an x
-// that is not finite in every row, 1.08 ms with a quarter of the requests on a NaN adapter or with all of low beyond fp16; summed again in scalars, 79 ms.
+// of the row's low is in fp16: it is the row's own then. The others are the row's x . w (kEpiAdapterF16; a warp's 32 x 16 of
+// them on mma.sync, its fragments as in thin_product_of) plus low . up of its own request. 3744 rows through 2048 x 2048, rank
+// 32, 50 us a call: 86 us with an x that is not finite in every row; 1.08 ms (int8 0.27 and 0.51) with a quarter of the
+// requests on a NaN adapter or with all of low beyond fp16, 79 ms when every such sum was taken again in scalars.
 template <int EPI>
 __device__ __noinline__ void take_sums_again(const AdapterGemmArgs& p, int m, int column, uint32_t* sums) {
     const int lane = threadIdx.x & 31, first_row = m - lane, tile_rows = p.adapters.tile_rows, tile = first_row / tile_rows, rank = p.adapters.rank;

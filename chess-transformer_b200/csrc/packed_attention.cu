@@ -25,9 +25,10 @@ FRY_DEVICE void cp_async16_or_zero(uint32_t shared, const void* global, bool rea
 // WIDTH: the head width padded to 32, 64 or 128 with zeros. KEY_WARPS: 1, the block's warps have 16 rows each and share the
 // keys; more, they have the same rows and KEYS keys each of a stage.
 //
-// What bounds them: the key warps HBM (64 full caches of 8192 keys, 8 heads of 128: 6.7 TB/s; of 2048, 12 heads of 64: 5.0 TB/s,
-// 4.5 with uneven lengths). The row warps the instructions: at 64 keys a stage, of 62 us for 256 x 70 tokens, 24 heads of 32, 20 go to the
-// search, the queries and the outputs, 13 to the copies and 29 to products and softmax.
+// What bounds them: the key warps HBM (64 full caches of 8192 keys, 8 heads of 128: 6.7 TB/s; of 2048, 12 heads of 64: 5.2
+// TB/s, 4.3 to 4.8 with uneven lengths). The row warps the instructions: of 59 us for 256 x 70 tokens, 24 heads of 32, 20 go
+// to the search, the queries and the outputs (no keys at all), 10 to the copies and 29 to products and softmax (256 x 64: 20, 6
+// and 21 of 47).
 constexpr int kMaxRowWarps = 8;
 template <int WIDTH, int KEY_WARPS, int KEYS, int STAGES>
 struct RowsShape {
@@ -368,7 +369,8 @@ cudaError_t launch_rows(AttentionArgs a, int row_warps, cudaStream_t stream) {
 }
 
 // Width 32, whose blocks have 64 registers a thread: 48 keys a stage spill less than 64 and waste less of a last stage (256 x
-// 70 tokens, 61.4 -> 58.2 us; 200 x 96, 64.9 -> 58.6; 700 x 24, 48.0 -> 44.5; but 256 x 64, 45.7 -> 46.5; 80: 67.9, 96: 73.0).
+// 70 tokens, 61.4 -> 58.2 us; 200 x 96, 64.9 -> 58.6; 700 x 24, 48.0 -> 44.5; of 70 tokens 80 keys 67.9 us, 96 73.0). Sequences
+// that fill one stage of 64 lose 2% by it (256 x 64, 45.7 -> 46.5 us).
 template <int WIDTH, bool BF16>
 cudaError_t launch_width(const AttentionArgs& a, const AttentionPlan& plan, cudaStream_t stream) {
     return plan.form == AttentionForm::kFew ? launch_rows<WIDTH, 4, 16, 3, BF16>(a, 1, stream) : launch_rows<WIDTH, 1, WIDTH == 32 ? 48 : 64, 2, BF16>(a, plan.row_warps, stream);
@@ -400,10 +402,13 @@ AttentionPlan attention_plan(const AttentionShape& s) {
     // rows and keys are filled well enough (64 x 64 tokens, 512 keys, 41 us against 59; x 128, 128 keys, 28 against 43; x 4
     // of 8 grouped heads, 2000 keys, 56 against 84 of the key warps; but 64 x 32 tokens, 256 keys, 28 against 22, and 128 x
     // 70 of 2 grouped heads, 70 keys, 80 against 52).
+    // One kernel takes the whole batch, the mean's: the host has no other length. A batch of like requests loses nothing, one
+    // prompt of 2000 tokens beside 255 single tokens after 2000 keys little (32/8 heads of 128: 406 us, 54 and 328 as two
+    // calls); one of 8192 beside 4000 sequences of one token and 3 keys takes 11.2 ms, 0.48 and 0.37 as two calls.
     const bool few = s.cached || (mean_rows <= 16 && mean_keys >= 128);
     const bool prompt = !few && mean_rows > 16 && mean_keys >= 128 && mean_rows * mean_keys >= 128 * 128;
     plan.form = few ? AttentionForm::kFew : prompt ? AttentionForm::kPrompt : AttentionForm::kRows;
-    // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more
+    // blocks without a split, and how many fit a round of the SMs twice over; a split keeps 256 keys or more of a mean sequence
     const int64_t group = s.heads / s.kv_heads;
     if (!few && !prompt) {
         // a mean sequence's rows in as few blocks as take them, spread evenly

@@ -7,8 +7,9 @@
 // tile are its softmax, a thread a row. Two tiles are on an SM, so that while one's scores are on the softmax the tensor
 // core works on the other's products: in two blocks of one, or in one block of two.
 // Two blocks start and end on their own, one's beginning and end under the other's work; one block's tiles share its key
-// and value stages, half the traffic from L2. Measured (two blocks / one): 8 x 512 tokens of 12 heads of 64 after ragged
-// keys 46.5 / 58.5 us, 16 prompts of 1000 tokens, 32 heads of 128, 232 / 244 us, one of 4096 151 / 154 us, of 8192 503 / 482 us.
+// and value stages, half the traffic from L2. Measured (five calls in a graph, device busy; two blocks / one): 8 x 512 tokens
+// of 12 heads of 64 after ragged keys 54 / 61 us; of 32 heads of 128, 16 prompts of 1000 tokens 228 / 236 us, one of 4096 141 /
+// 138, of 5000 198 / 201, of 6144 290 / 289, of 7000 399 / 373, of 8192 535 / 502 (the power cap moves these by 5%).
 // What bounds it: a step of both tiles (2 x 128 rows by 128 keys) takes about 3400 clocks at width 128, of which the
 // tensor core is busy for 2048 and the exponentials (16 a clock and SM) for 2048. A row tile's chain of loads from TMEM
 // (250 clocks), exponentials (64 at a time 520 to 900, with the other tile at its own), hand-over and products (1100)

@@ -127,9 +127,10 @@ int fry_attention_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
  * outside their tensor or descending are read as the nearest row and recorded (code 7, where = the sequence); what the
  * rows then hold is unspecified. out [q_rows, heads, head_dim] is dense and overlaps no input; strides are in elements,
  * multiples of 8, the last axis dense; q, k, v and out 16-byte aligned. head_dim a multiple of 8 up to 128, heads a multiple of
- * kv_heads up to 1024, query rows and sequences below 2^24, key rows up to 2^30, scale positive, up to 2e38. workspace: 16-byte aligned, of fry_packed_attention_workspace_bytes (0 where the
- * keys are not split over blocks). Calls whose work overlaps on the GPU need workspaces of their own. The reference has
- * no attention of this form: its template attention (model/fused_blocks.py:54-97) sees 70 tokens, all of them. */
+ * kv_heads up to 1024, query rows and sequences below 2^24, key rows up to 2^30, scale positive, up to 2e38. workspace: 16-byte
+ * aligned, of fry_packed_attention_workspace_bytes (0 where the keys are not split over blocks). Calls whose work overlaps on
+ * the GPU need workspaces of their own. The reference has no attention of this form: its template attention
+ * (model/fused_blocks.py:54-97) sees 70 tokens, all of them. */
 size_t fry_packed_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim);
 int fry_packed_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int32_t* q_offsets,
                          const int32_t* k_offsets, int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim,
