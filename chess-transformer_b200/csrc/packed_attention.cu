@@ -179,7 +179,7 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
                 if (n % 2 == 0 && n * 8 >= left) break;
                 top = max3(top, s[n][2 * half], s[n][2 * half + 1]);
             }
-            top = fmaxf(m[half], quad_max(top) * a.scale_log2);
+            top = fmaxf(m[half], __fmul_rn(quad_max(top), a.scale_log2));
             const float base = top == -INFINITY ? 0.0f : top, shrink = ex2_approx_ftz(m[half] - base);
             m[half] = top;
             l[half] *= shrink;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__((RowsShape<WIDTH, KEY_WARPS, KEYS, STAGES>::kM
 #pragma unroll
             for (int n = 0; n < KEYS / 8; ++n) {
                 if (n % 2 == 0 && n * 8 >= left) break;
-                const float2 x = lanes(fma2(pair2(s[n][2 * half], s[n][2 * half + 1]), scale2, base2));
+                const float2 x = lanes(add2(product2(pair2(s[n][2 * half], s[n][2 * half + 1]), scale2), base2));
                 s[n][2 * half] = ex2_approx_ftz(x.x), s[n][2 * half + 1] = ex2_approx_ftz(x.y);
                 total2 = add2(total2, pair2(s[n][2 * half], s[n][2 * half + 1]));
             }

@@ -10,8 +10,8 @@
 // Softmax in one pass over the keys: with m the running maximum of a row's scores (times scale log2 e) and l the running
 // sum of 2^(s - m), a tile of keys takes m to m' = max(m, its maximum), scales l and the row's sums o by 2^(m - m') and
 // adds its own 2^(s - m') and 2^(s - m') v. out = o / l at the end; a row that sees no key has l = 0 and answers 0. Scores,
-// m, l and o are fp32. The probabilities 2^(s - m') are rounded to the inputs' type for the second product (off by at most
-// half a step each, about what rounding the output costs), l sums them unrounded.
+// m, l and o are fp32. The probabilities 2^(s - m') are rounded to the inputs' type for the second product (off by at most half a
+// step each, about what rounding the output costs), l sums them unrounded.
 //
 // Rows. The `group` query heads of a key/value head share its keys, so they are rows of one tile: row r of a block is token
 // r / group, head r % group, and one pass over the keys serves them all.
@@ -126,6 +126,15 @@ FRY_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uin
     if constexpr (BF16) mma_bf16(c, a, b0, b1);
     else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
 }
+
+// Whether a running maximum is so large that its rounding shows in the exponentials: s - m' as one FMA of the raw score, the
+// scale and m' keeps the largest score's own rounding, up to half a step of m'. Below 2^22 that is 1/4 at most and alike for
+// all of a row's weights; from 2^30 on it makes the largest probability 0 or infinite. There scores are scaled and rounded
+// first, as m' was. The row kernels do so for all (product2; 1%), the prompts, which it would cost 2 to 5%, ask first (1 to 2%).
+// product2: in mul.rn.f32x2 and add.rn.f32x2 one behind the other the product comes out in an FMA with the sum, and a zero
+// addend keeps them apart.
+FRY_DEVICE uint64_t product2(uint64_t a, uint64_t b) { return fma2(a, b, pair2(0.0f, 0.0f)); }
+FRY_DEVICE bool rounds_apart(float m) { return fabsf(m) >= 4194304.0f && m != -INFINITY; }
 
 FRY_DEVICE float max3(float a, float b, float c) {
     float m;
@@ -294,8 +303,8 @@ __device__ __noinline__ void repair_rows(const AttentionArgs& a, RowBlock b, uin
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int j = j0 + 8 * n + 2 * t;
-                        const float even = ex2_approx_ftz(__fmaf_rn(s[n][2 * half], a.scale_log2, -base[half]));
-                        const float odd = ex2_approx_ftz(__fmaf_rn(s[n][2 * half + 1], a.scale_log2, -base[half]));
+                        const float even = ex2_approx_ftz(__fsub_rn(__fmul_rn(s[n][2 * half], a.scale_log2), base[half]));
+                        const float odd = ex2_approx_ftz(__fsub_rn(__fmul_rn(s[n][2 * half + 1], a.scale_log2), base[half]));
                         p[2 * n + half] = pack16<BF16>(j < limit[half] ? even : 0.0f, j + 1 < limit[half] ? odd : 0.0f);
                     }
 #pragma unroll

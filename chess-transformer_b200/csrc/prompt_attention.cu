@@ -268,7 +268,8 @@ __global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (Prompt
         const uint32_t lanes_at = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_tmem = tmem + t * kPromptTile + lanes_at, o_tmem = tmem + S::kOutAt + t * WIDTH + lanes_at;
         const uint32_t p_tmem = tmem + S::kProbabilitiesAt + t * S::kProbabilities + lanes_at;
-        const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2);
+        float scale = a.scale_log2;  // 1 once scores are scaled apart
+        bool apart = false;
         float m = -INFINITY;
         uint64_t totals[2] = {pair2(0.0f, 0.0f), pair2(0.0f, 0.0f)};
         bool alive = true;
@@ -314,13 +315,13 @@ __global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (Prompt
 #pragma unroll
                     for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(raw[c][e]), __uint_as_float(raw[c][e + 1]));
                 }
-                return fmaxf(m, max3(top[0], top[1], fmaxf(top[2], top[3])) * a.scale_log2);
+                return fmaxf(m, __fmul_rn(max3(top[0], top[1], fmaxf(top[2], top[3])), scale));
             };
             uint32_t packed[32];
             uint64_t sums[2];
             auto probabilities = [&](int half) {  // of 64 keys, and their sums
                 const float base = m == -INFINITY ? 0.0f : -m;
-                const uint64_t base2 = pair2(base, base);
+                const uint64_t base2 = pair2(base, base), scale2 = pair2(scale, scale);
                 sums[0] = sums[1] = pair2(0.0f, 0.0f);
 #pragma unroll
                 for (int e = 0; e < 64; e += 2) {
@@ -340,7 +341,15 @@ __global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (Prompt
                 if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
                 __syncwarp();  // together again before the next warp-wide TMEM access
             };
-            if (j == 0) m = highest();
+            auto scale_apart = [&] {
+                scale = 1.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) raw[c][e] = __float_as_uint(__fmul_rn(__uint_as_float(raw[c][e]), a.scale_log2));
+            };
+            if (j == 0) m = highest(), apart = __any_sync(0xffffffffu, rounds_apart(m));
+            if (apart) scale_apart();
             probabilities(0);
             const float risen = highest();
             // P V of the keys before is done: at width 128 the scores came after it
@@ -348,6 +357,7 @@ __global__ void __launch_bounds__((PromptShape<WIDTH, TILES>::kThreads), (Prompt
             if (__any_sync(0xffffffffu, risen > m + kLagLog2)) {
                 const float shrink = risen == -INFINITY ? 0.0f : ex2_approx_ftz(m - risen);
                 m = risen;
+                if (!apart && __any_sync(0xffffffffu, rounds_apart(m))) apart = true, scale_apart();
                 totals[0] = mul2(totals[0], pair2(shrink, shrink)), totals[1] = mul2(totals[1], pair2(shrink, shrink));
                 tc_fence_after();
 #pragma unroll 1
