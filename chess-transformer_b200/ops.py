@@ -204,7 +204,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     device). Causal, its queries are its last tokens: query i of nq sees keys j <= i + nk - nq. Rows that see no key, and
     rows of no sequence, are 0. width a multiple of 8 up to 128; scale defaults to 1 / sqrt(width). No backward pass.
     Strided views (of a projection's rows, say) are read in place where their last axis is dense and their other strides
-    are multiples of 8."""
+    are multiples of 8 other than 0; others are copied first."""
     q_shape, k_shape, dtype, index = q.shape, k.shape, q.dtype, q.get_device()
     shaped = (len(q_shape) == 3 and len(k_shape) == 3 and v.shape == k_shape and q_shape[2] == k_shape[2] and k_shape[1] > 0
               and q_shape[1] % k_shape[1] == 0)
